@@ -471,6 +471,90 @@ int l3g_gemm_q8(const l3g_gemm_matrix *w, const void *act, int32_t n_tok,
                 float *out, void *stream);
 int l3g_gemm_status(const l3g_gemm_matrix *w, int32_t *err, int32_t *where);
 
+/* ---- serving operators ---------------------------------------------------- */
+/* None of these has a counterpart in the reference, which runs one session a
+ * token at a time (cmd/go-llama-chat/main.go:139-176).  DEVICE pointers unless
+ * said otherwise, 16-byte aligned; calls are asynchronous on `stream` and keep
+ * the caller's current device.  The calls of one handle share its scratch, so
+ * they must not overlap in time (one stream, or ordered ones); that holds for
+ * replays of graphs that captured them too.  A call allocates nothing and can
+ * be captured. */
+
+/* Attention of chunks of new tokens over paged caches.  Sequence s has n_q new
+ * tokens, rows q0 .. q0 + n_q - 1 of q and out, and a cache of kv_len
+ * positions that holds them already as its last n_q; token i sees the
+ * positions 0 .. kv_len - n_q + i:
+ *   out = sum_j softmax_j(scale * q . K_j) V_j   (infer.go:130-175 per token).
+ * A token that sees no position (kv_len < n_q leaves such) gets zeros.  Query
+ * head h reads kv head h / (n_heads / n_heads_kv).  Rows of q and out that no
+ * sequence names are not touched; the sequences' rows must not overlap. */
+typedef struct {
+  const void *pool;     /* page 0 of its pool: pages of [L3G_KV_PAGE][K | V] rows */
+  const int32_t *pages; /* its page table: position p of (layer, kv head) is in
+                           page [(layer * n_heads_kv + kv head) * pps + p / L3G_KV_PAGE] */
+  int32_t n_pages;      /* pages of the pool                                    */
+  int32_t pps;          /* page-table entries per (layer, kv head)               */
+  int32_t q0, n_q;      /* its rows of q and out                                 */
+  int32_t kv_len;       /* positions of its cache, the new tokens included       */
+  int32_t pad;
+} l3g_chunk_seq;
+typedef struct l3g_chunk_attn l3g_chunk_attn;
+/* head_dim 32, 64 or 128; n_heads / n_heads_kv at most 8; kv_dtype L3G_KV_*. */
+int l3g_chunk_attn_new(int32_t n_heads, int32_t n_heads_kv, int32_t head_dim,
+                       int32_t kv_dtype, int32_t device, l3g_chunk_attn **out);
+void l3g_chunk_attn_free(l3g_chunk_attn *h);
+/* seqs: n_seqs descriptors (DEVICE, at most L3G_CHUNK_SEQS_MAX); total_q rows
+ * of q (f32 [n_heads][head_dim] at q + row * ldq) and out (ldo), row strides in
+ * floats, multiples of 4; layer selects the page-table rows; scale <= 0 means
+ * 1 / sqrt(head_dim).  A descriptor outside its bounds (rows, kv_len, a page
+ * id) is skipped, its rows left as they were (for a bad page: those of the
+ * head's tokens that see it, at least), and noted for l3g_chunk_attn_status.
+ * A NaN or an infinity in K or V gives NaN in the rows that see it and touches
+ * no other. */
+#define L3G_CHUNK_SEQS_MAX 1024
+int l3g_chunk_attn_run(l3g_chunk_attn *h, const l3g_chunk_seq *seqs,
+                       int32_t n_seqs, int32_t total_q, const float *q,
+                       int64_t ldq, float *out, int64_t ldo, int32_t layer,
+                       float scale, void *stream);
+/* Synchronizes the device, returns and clears the error word of the calls so
+ * far: err 0; 1 a bounded wait gave up (`where` names it); 3 sequence `where`
+ * outside its bounds; 4 page id `where` outside its pool. */
+int l3g_chunk_attn_status(l3g_chunk_attn *h, int32_t *err, int32_t *where);
+
+/* Log probabilities of given tokens, entropy, rank and top alternatives of n
+ * rows of f32 logits (row r at logits + r * ld, vocab values):
+ *   logprob[r] = x_t - lse, t = targets[r], lse = log sum_i exp(x_i);
+ *   entropy[r] = - sum_i p_i log p_i, p_i = exp(x_i - lse)  (nats);
+ *   rank[r]    = tokens that come before t by (logit descending, id ascending);
+ *   top_ids, top_logprobs [n][top_k]: the first top_k tokens in that order
+ * (the order of ForwardTopKIntoWorkspace's items, topk.go).  -inf logits are
+ * tokens of probability zero; a row of nothing else has entropy 0 and log
+ * probabilities of -inf.  A row with a NaN or +inf has NaN for logprob, entropy
+ * and top_logprobs, and in its order NaNs follow their sign bits beyond the
+ * infinities.  A target outside [0, vocab) is none: logprob NaN, rank -1.
+ * logprob and rank (with targets), entropy, top_ids and top_logprobs may be
+ * NULL; top_k in [0, 64], at most vocab.  ld >= vocab. */
+typedef struct l3g_logprobs l3g_logprobs;
+int l3g_logprobs_new(int32_t max_rows, int32_t vocab, int32_t device,
+                     l3g_logprobs **out);
+void l3g_logprobs_free(l3g_logprobs *h);
+int l3g_logprobs_run(l3g_logprobs *h, const float *logits, int64_t ld,
+                     int32_t n, const int32_t *targets, float *logprob,
+                     float *entropy, int32_t *rank, int32_t top_k,
+                     int32_t *top_ids, float *top_logprobs, void *stream);
+
+/* Copies rows between pages: for i < n the first rows[i] rows (rows NULL: all
+ * L3G_KV_PAGE) of page src[i] of src_pool to page dst[i] of dst_pool; a page is
+ * L3G_KV_PAGE rows of row_bytes (a multiple of 16), n_src and n_dst pages per
+ * pool.  Destinations are distinct, and none is read by the call.  An entry
+ * outside its bounds is skipped; *status (int32 x 2, nullable, cleared by its
+ * owner) then holds 4 and the entry's index.  The pools are on the device that
+ * is current. */
+int l3g_kv_copy_pages(const void *src_pool, int32_t n_src, void *dst_pool,
+                      int32_t n_dst, int32_t row_bytes, const int32_t *src,
+                      const int32_t *dst, const int32_t *rows, int32_t n,
+                      int32_t *status, void *stream);
+
 /* ---- inspection (tests, debugging) --------------------------------------- */
 /* KV entries of one layer for positions [pos0, pos0+npos) in the reference
  * layout [pos][kv_head][head_dim] (f32, host), this rank's kv heads only. */

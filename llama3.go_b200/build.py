@@ -19,7 +19,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libl3g.so")
 UNITS = ["l3g_api.cu", "l3g_model.cu", "l3g_tp.cu", "l3g_step.cu", "l3g_persist_host.cu",
-         "l3g_batched.cu", "l3g_gguf.cpp"]
+         "l3g_batched.cu", "l3g_ops.cu", "l3g_gguf.cpp"]
 OBJDIR = os.path.join(HERE, "_build")
 
 

@@ -20,7 +20,7 @@ constexpr int MAX_TOPK = 64;  // largest top-K a workspace serves
 constexpr unsigned long long WAIT_TIMEOUT_PEER_NS = 30000000000ull;  // 30 s
 
 // device error codes (Result::err); Result::where names the wait site
-enum { ERR_NONE = 0, ERR_TIMEOUT = 1, ERR_TOKEN = 2 };
+enum { ERR_NONE = 0, ERR_TIMEOUT = 1, ERR_TOKEN = 2, ERR_SEQ = 3, ERR_PAGE = 4 };
 
 struct Result {        // copied to the host at the end of every step
   int32_t token;       // argmax id (greedy)

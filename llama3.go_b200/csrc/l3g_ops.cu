@@ -1,0 +1,233 @@
+// The serving operators: attention of token chunks over paged caches, log
+// probabilities, page copies.
+#include "l3g_rt.h"
+
+namespace l3g {
+#include "l3g_chunk_attn.cuh"
+
+#include "l3g_logprobs.cuh"
+
+#include "l3g_pages.cuh"
+}  // namespace l3g
+
+// Makes `dev` current for a call and puts the caller's device back.
+struct DeviceScope {
+  int prev = -1;
+  cudaError_t err = cudaSuccess;
+  explicit DeviceScope(int dev) {
+    err = cudaGetDevice(&prev);
+    if (err == cudaSuccess && prev != dev) err = cudaSetDevice(dev);
+    if (prev == dev) prev = -1;
+  }
+  ~DeviceScope() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+#define ON_DEVICE(dev)      \
+  DeviceScope scope_(dev);  \
+  CUDA_TRY(scope_.err)
+
+static bool misaligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) != 0; }
+
+// ---------------------------------------------------------------------------
+// attention of token chunks
+// ---------------------------------------------------------------------------
+struct l3g_chunk_attn {
+  int device = 0, nsm = 1;
+  int heads = 0, hkv = 0, hd = 0, kv_f16 = 0;
+  Result* d_res = nullptr;
+};
+
+extern "C" void l3g_chunk_attn_free(l3g_chunk_attn* h) {
+  if (!h) return;
+  DeviceScope scope(h->device);
+  if (h->d_res) cudaFree(h->d_res);
+  delete h;
+}
+
+extern "C" int l3g_chunk_attn_new(int32_t n_heads, int32_t n_heads_kv, int32_t head_dim,
+                                  int32_t kv_dtype, int32_t device, l3g_chunk_attn** out) {
+  if (!out) return l3g_fail(L3G_E_INVALID, "null argument");
+  *out = nullptr;
+  if (n_heads <= 0 || n_heads_kv <= 0 || n_heads % n_heads_kv || n_heads / n_heads_kv > MAXG ||
+      n_heads_kv > 65535)
+    return l3g_fail(L3G_E_INVALID, "chunk attention: %d query heads over %d kv heads", n_heads,
+                    n_heads_kv);
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128)
+    return l3g_fail(L3G_E_INVALID, "chunk attention: head_dim %d", head_dim);
+  if (kv_dtype != L3G_KV_F32 && kv_dtype != L3G_KV_F16)
+    return l3g_fail(L3G_E_INVALID, "kv_dtype=%d", kv_dtype);
+  int dev = device;
+  if (dev < 0) CUDA_TRY(cudaGetDevice(&dev));
+  ON_DEVICE(dev);
+  auto* h = new l3g_chunk_attn();
+  h->device = dev;
+  h->nsm = sm_count(dev);
+  h->heads = n_heads;
+  h->hkv = n_heads_kv;
+  h->hd = head_dim;
+  h->kv_f16 = kv_dtype == L3G_KV_F16;
+  cudaError_t e = cudaMalloc(&h->d_res, sizeof(Result));
+  if (e == cudaSuccess) e = cudaMemset(h->d_res, 0, sizeof(Result));
+  if (e != cudaSuccess) {
+    l3g_chunk_attn_free(h);
+    return l3g_fail(L3G_E_CUDA, "chunk attention: %s", cudaGetErrorString(e));
+  }
+  *out = h;
+  return L3G_OK;
+}
+
+template <int HD, typename KT>
+static cudaError_t launch_chunk(const l3g_chunk_attn* h, const ChunkArgs& a, cudaStream_t st) {
+  const long long blocks = ((long long)a.total_q * a.heads + 7) / 8;
+  k_chunk_simple<HD, KT>
+      <<<dim3((unsigned)std::min<long long>(blocks, 8LL * h->nsm), a.n_seqs), 256, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+extern "C" int l3g_chunk_attn_run(l3g_chunk_attn* h, const l3g_chunk_seq* seqs, int32_t n_seqs,
+                                  int32_t total_q, const float* q, int64_t ldq, float* out,
+                                  int64_t ldo, int32_t layer, float scale, void* stream) {
+  if (!h) return l3g_fail(L3G_E_INVALID, "null argument");
+  if (n_seqs < 0 || n_seqs > L3G_CHUNK_SEQS_MAX)
+    return l3g_fail(L3G_E_INVALID, "n_seqs=%d outside [0, %d]", n_seqs, L3G_CHUNK_SEQS_MAX);
+  if (total_q < 0 || layer < 0)
+    return l3g_fail(L3G_E_INVALID, "total_q=%d, layer=%d", total_q, layer);
+  if (n_seqs == 0 || total_q == 0) return L3G_OK;
+  if (!seqs || !q || !out) return l3g_fail(L3G_E_INVALID, "null argument");
+  const int64_t width = (int64_t)h->heads * h->hd;
+  if (ldq < width || ldo < width || ldq % 4 || ldo % 4)
+    return l3g_fail(L3G_E_INVALID, "row strides %lld and %lld: multiples of 4, at least %lld",
+                    (long long)ldq, (long long)ldo, (long long)width);
+  if (misaligned(q, 16) || misaligned(out, 16) || misaligned(seqs, 8))
+    return l3g_fail(L3G_E_INVALID, "q and out must be 16-byte aligned, seqs 8-byte");
+  if (std::isnan(scale) || std::isinf(scale)) return l3g_fail(L3G_E_INVALID, "scale not finite");
+  ON_DEVICE(h->device);
+  ChunkArgs a{};
+  a.seqs = seqs;
+  a.n_seqs = n_seqs;
+  a.total_q = total_q;
+  a.q = q;
+  a.ldq = ldq;
+  a.out = out;
+  a.ldo = ldo;
+  a.layer = layer;
+  a.heads = h->heads;
+  a.hkv = h->hkv;
+  a.group = h->heads / h->hkv;
+  a.scale = scale > 0.0f ? scale : (float)(1.0 / sqrt((double)h->hd));
+  a.res = h->d_res;
+  const cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t e;
+  if (h->kv_f16)
+    e = h->hd == 32 ? launch_chunk<32, __half>(h, a, st)
+                    : h->hd == 64 ? launch_chunk<64, __half>(h, a, st)
+                                  : launch_chunk<128, __half>(h, a, st);
+  else
+    e = h->hd == 32 ? launch_chunk<32, float>(h, a, st)
+                    : h->hd == 64 ? launch_chunk<64, float>(h, a, st)
+                                  : launch_chunk<128, float>(h, a, st);
+  CUDA_TRY(e);
+  return L3G_OK;
+}
+
+extern "C" int l3g_chunk_attn_status(l3g_chunk_attn* h, int32_t* err, int32_t* where) {
+  if (!h || !err || !where) return l3g_fail(L3G_E_INVALID, "null argument");
+  ON_DEVICE(h->device);
+  CUDA_TRY(cudaDeviceSynchronize());
+  Result r{};
+  CUDA_TRY(cudaMemcpy(&r, h->d_res, sizeof r, cudaMemcpyDeviceToHost));
+  CUDA_TRY(cudaMemset(h->d_res, 0, sizeof(Result)));
+  *err = r.err;
+  *where = r.where;
+  return L3G_OK;
+}
+
+// ---------------------------------------------------------------------------
+// log probabilities
+// ---------------------------------------------------------------------------
+struct l3g_logprobs {
+  int device = 0, nsm = 1;
+  int max_rows = 0, vocab = 0;
+};
+
+extern "C" void l3g_logprobs_free(l3g_logprobs* h) { delete h; }
+
+extern "C" int l3g_logprobs_new(int32_t max_rows, int32_t vocab, int32_t device,
+                                l3g_logprobs** out) {
+  if (!out) return l3g_fail(L3G_E_INVALID, "null argument");
+  *out = nullptr;
+  if (max_rows <= 0 || max_rows > (1 << 20) || vocab <= 0 || vocab > (1 << 24))
+    return l3g_fail(L3G_E_INVALID, "log probabilities of %d rows of %d", max_rows, vocab);
+  int dev = device;
+  if (dev < 0) CUDA_TRY(cudaGetDevice(&dev));
+  ON_DEVICE(dev);
+  auto* h = new l3g_logprobs();
+  h->device = dev;
+  h->nsm = sm_count(dev);
+  h->max_rows = max_rows;
+  h->vocab = vocab;
+  *out = h;
+  return L3G_OK;
+}
+
+extern "C" int l3g_logprobs_run(l3g_logprobs* h, const float* logits, int64_t ld, int32_t n,
+                                const int32_t* targets, float* logprob, float* entropy,
+                                int32_t* rank, int32_t top_k, int32_t* top_ids,
+                                float* top_logprobs, void* stream) {
+  if (!h) return l3g_fail(L3G_E_INVALID, "null argument");
+  if (n < 0 || n > h->max_rows)
+    return l3g_fail(L3G_E_INVALID, "n=%d outside [0, %d]", n, h->max_rows);
+  if (top_k < 0 || top_k > MAX_TOPK || top_k > h->vocab)
+    return l3g_fail(L3G_E_INVALID, "top_k=%d outside [0, %d]", top_k,
+                    std::min(MAX_TOPK, h->vocab));
+  if (ld < h->vocab)
+    return l3g_fail(L3G_E_INVALID, "row stride %lld below the vocabulary %d", (long long)ld,
+                    h->vocab);
+  if (n == 0) return L3G_OK;
+  if (!logits || (!targets && (logprob || rank)))
+    return l3g_fail(L3G_E_INVALID, "null argument");
+  const void* ps[] = {logits, targets, logprob, entropy, rank, top_ids, top_logprobs};
+  for (const void* p : ps)
+    if (misaligned(p, 4)) return l3g_fail(L3G_E_INVALID, "pointers must be 4-byte aligned");
+  if (!top_ids && !top_logprobs) top_k = 0;
+  ON_DEVICE(h->device);
+  LogprobArgs a{};
+  a.x = logits;
+  a.ld = ld;
+  a.n = n;
+  a.vocab = h->vocab;
+  a.k = top_k;
+  a.targets = targets;
+  a.logprob = logprob;
+  a.entropy = entropy;
+  a.rank = rank;
+  a.top_ids = top_ids;
+  a.top_lp = top_logprobs;
+  k_logprobs_simple<<<n, 256, 0, (cudaStream_t)stream>>>(a);
+  CUDA_TRY(cudaGetLastError());
+  return L3G_OK;
+}
+
+// ---------------------------------------------------------------------------
+// page copies
+// ---------------------------------------------------------------------------
+extern "C" int l3g_kv_copy_pages(const void* src_pool, int32_t n_src, void* dst_pool,
+                                 int32_t n_dst, int32_t row_bytes, const int32_t* src,
+                                 const int32_t* dst, const int32_t* rows, int32_t n,
+                                 int32_t* status, void* stream) {
+  if (n < 0 || n_src < 0 || n_dst < 0)
+    return l3g_fail(L3G_E_INVALID, "n=%d, pools of %d and %d pages", n, n_src, n_dst);
+  if (row_bytes <= 0 || row_bytes % 16 || row_bytes > 65536)
+    return l3g_fail(L3G_E_INVALID, "rows of %d bytes: a multiple of 16, at most 65536", row_bytes);
+  if (n == 0) return L3G_OK;
+  if (!src_pool || !dst_pool || !src || !dst) return l3g_fail(L3G_E_INVALID, "null argument");
+  if (misaligned(src_pool, 16) || misaligned(dst_pool, 16) || misaligned(src, 4) ||
+      misaligned(dst, 4) || misaligned(rows, 4) || misaligned(status, 4))
+    return l3g_fail(L3G_E_INVALID, "pools must be 16-byte aligned, arrays 4-byte");
+  k_copy_pages<<<dim3(4, std::min(n, 65535)), 256, 0, (cudaStream_t)stream>>>(
+      static_cast<const uint8_t*>(src_pool), n_src, static_cast<uint8_t*>(dst_pool), n_dst,
+      row_bytes, src, dst, rows, n, status);
+  CUDA_TRY(cudaGetLastError());
+  return L3G_OK;
+}

@@ -1,0 +1,23 @@
+// Copies between pages of a KV cache (included by l3g_ops.cu inside namespace
+// l3g).
+#pragma once
+
+// Entry i copies rows [0, rows[i]) of page src[i] to page dst[i], 16 bytes a
+// thread and step.  grid (x: slices of an entry, y: entries).
+static __global__ void k_copy_pages(const uint8_t* sp, int n_src, uint8_t* dp, int n_dst,
+                                    int row_bytes, const int* src, const int* dst,
+                                    const int* rows, int n, int* status) {
+  for (int i = blockIdx.y; i < n; i += gridDim.y) {
+    const int s = src[i], d = dst[i], r = rows ? rows[i] : KV_PAGE;
+    if (s < 0 || s >= n_src || d < 0 || d >= n_dst || r < 0 || r > KV_PAGE) {
+      if (status && threadIdx.x == 0 && blockIdx.x == 0 && atomicCAS(status, 0, ERR_PAGE) == 0)
+        atomicExch(status + 1, i);
+      continue;
+    }
+    const int4* a = reinterpret_cast<const int4*>(sp + (size_t)s * KV_PAGE * row_bytes);
+    int4* b = reinterpret_cast<int4*>(dp + (size_t)d * KV_PAGE * row_bytes);
+    const int m = r * (row_bytes >> 4);
+    for (int e = blockIdx.x * blockDim.x + threadIdx.x; e < m; e += gridDim.x * blockDim.x)
+      b[e] = a[e];
+  }
+}

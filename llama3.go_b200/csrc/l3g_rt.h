@@ -8,7 +8,8 @@
 // l3g_tp.cu (tensor-parallel exchange set-up), l3g_step.cu (workspaces,
 // the per-step graphs and every per-token entry, the matrix entries),
 // l3g_persist_host.cu (the persistent layer kernel), l3g_batched.cu (the
-// tensor-core product, batched prefill, batched decode).  A kernel is set
+// tensor-core product, batched prefill, batched decode), l3g_ops.cu (the
+// serving operators).  A kernel is set
 // up (attributes) and launched in the same unit: each unit is its own
 // device module.
 #pragma once

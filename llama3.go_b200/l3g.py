@@ -156,6 +156,17 @@ def lib():
         "l3g_gemm_quantize": (C.c_int, [_P, C.c_int32, C.c_int32, _P, _P]),
         "l3g_gemm_q8": (C.c_int, [_P, _P, C.c_int32, _P, _P]),
         "l3g_gemm_status": (C.c_int, [_P, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
+        "l3g_chunk_attn_new": (C.c_int, [C.c_int32] * 5 + [C.POINTER(_P)]),
+        "l3g_chunk_attn_free": (None, [_P]),
+        "l3g_chunk_attn_run": (C.c_int, [_P, _P, C.c_int32, C.c_int32, _P, C.c_int64, _P, C.c_int64,
+                                         C.c_int32, C.c_float, _P]),
+        "l3g_chunk_attn_status": (C.c_int, [_P, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
+        "l3g_logprobs_new": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.POINTER(_P)]),
+        "l3g_logprobs_free": (None, [_P]),
+        "l3g_logprobs_run": (C.c_int, [_P, _P, C.c_int64, C.c_int32, _P, _P, _P, _P, C.c_int32, _P, _P,
+                                       _P]),
+        "l3g_kv_copy_pages": (C.c_int, [_P, C.c_int32, _P, C.c_int32, C.c_int32, _P, _P, _P, C.c_int32,
+                                        _P, _P]),
         "l3g_state_read_kv": (C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32,
                                         C.POINTER(C.c_float), C.POINTER(C.c_float)]),
         "l3g_workspace_read": (C.c_int, [_P, C.c_int32, C.POINTER(C.c_float), C.c_int32]),
@@ -757,6 +768,92 @@ class GemmMatrix:
             self.Close()
         except Exception:
             pass
+
+
+# l3g_chunk_seq: one sequence of a chunk attention call
+CHUNK_SEQ = np.dtype([("pool", np.uint64), ("pages", np.uint64), ("n_pages", np.int32), ("pps", np.int32),
+                      ("q0", np.int32), ("n_q", np.int32), ("kv_len", np.int32), ("pad", np.int32)])
+
+
+def chunk_seqs(n: int) -> np.ndarray:
+    """n zeroed sequence descriptors (CHUNK_SEQ); fill them and copy their
+    bytes to the device for ChunkAttention.run."""
+    return np.zeros(n, CHUNK_SEQ)
+
+
+class ChunkAttention:
+    """Attention of ragged chunks of new tokens over paged caches
+    (l3g_chunk_attn): the handle owns the call's scratch, so its calls must
+    not overlap in time."""
+
+    def __init__(self, n_heads: int, n_heads_kv: int, head_dim: int, kv_dtype: int = L3G_KV_F32,
+                 device: int = -1):
+        h = C.c_void_p()
+        _check(lib().l3g_chunk_attn_new(n_heads, n_heads_kv, head_dim, kv_dtype, device, C.byref(h)))
+        self._h = h
+
+    def run(self, seqs_ptr: int, n_seqs: int, total_q: int, q_ptr: int, ldq: int, out_ptr: int, ldo: int,
+            layer: int = 0, scale: float = 0.0, stream: int = 0):
+        """Device pointers; q and out rows of n_heads * head_dim floats at
+        strides ldq and ldo, seqs_ptr n_seqs CHUNK_SEQ descriptors."""
+        _check(lib().l3g_chunk_attn_run(self._h, seqs_ptr, n_seqs, total_q, q_ptr, ldq, out_ptr, ldo, layer,
+                                        scale, stream or None))
+
+    def status(self):
+        """(err, where) of the calls since the last status()."""
+        e, w = C.c_int32(), C.c_int32()
+        _check(lib().l3g_chunk_attn_status(self._h, C.byref(e), C.byref(w)))
+        return e.value, w.value
+
+    def Close(self):
+        if self._h:
+            lib().l3g_chunk_attn_free(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.Close()
+        except Exception:
+            pass
+
+
+class LogProbs:
+    """Log probabilities of given tokens with entropy, rank and top
+    alternatives over rows of logits (l3g_logprobs); calls of one handle must
+    not overlap in time."""
+
+    def __init__(self, max_rows: int, vocab: int, device: int = -1):
+        h = C.c_void_p()
+        _check(lib().l3g_logprobs_new(max_rows, vocab, device, C.byref(h)))
+        self._h = h
+
+    def run(self, logits_ptr: int, ld: int, n: int, targets_ptr: int = 0, logprob_ptr: int = 0,
+            entropy_ptr: int = 0, rank_ptr: int = 0, top_k: int = 0, top_ids_ptr: int = 0,
+            top_logprobs_ptr: int = 0, stream: int = 0):
+        """Device pointers (0: not wanted); n rows of logits at stride ld."""
+        _check(lib().l3g_logprobs_run(self._h, logits_ptr or None, ld, n, targets_ptr or None,
+                                      logprob_ptr or None, entropy_ptr or None, rank_ptr or None, top_k,
+                                      top_ids_ptr or None, top_logprobs_ptr or None, stream or None))
+
+    def Close(self):
+        if self._h:
+            lib().l3g_logprobs_free(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.Close()
+        except Exception:
+            pass
+
+
+def kv_copy_pages(src_pool_ptr: int, n_src: int, dst_pool_ptr: int, n_dst: int, row_bytes: int, src_ptr: int,
+                  dst_ptr: int, rows_ptr: int, n: int, status_ptr: int = 0, stream: int = 0):
+    """The first rows[i] rows (rows_ptr 0: all) of page src[i] to page dst[i]
+    for i < n, device pointers (l3g_kv_copy_pages)."""
+    _check(lib().l3g_kv_copy_pages(src_pool_ptr or None, n_src, dst_pool_ptr or None, n_dst, row_bytes,
+                                   src_ptr or None, dst_ptr or None, rows_ptr or None, n, status_ptr or None,
+                                   stream or None))
 
 
 def quantize_q8_0_device(x_ptr: int, n: int, d_ptr: int, qs_ptr: int, stream: int = 0):
