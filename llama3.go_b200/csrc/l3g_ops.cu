@@ -3,6 +3,8 @@
 #include "l3g_rt.h"
 
 namespace l3g {
+#include "l3g_tc16.cuh"
+
 #include "l3g_chunk_attn.cuh"
 
 #include "l3g_logprobs.cuh"
@@ -36,12 +38,45 @@ struct l3g_chunk_attn {
   int device = 0, nsm = 1;
   int heads = 0, hkv = 0, hd = 0, kv_f16 = 0;
   Result* d_res = nullptr;
+  float* part_o = nullptr;   // pieces of row tiles that several CTAs share
+  float* part_ml = nullptr;
+  int* split = nullptr;
 };
+
+// Kernel attributes, once per device, with that device current.
+static int chunk_setup() {
+  static int rcs[64];
+  static std::once_flag onces[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
+    return l3g_fail(L3G_E_CUDA, "chunk attention set-up: no current device");
+  int& rc = rcs[dev];
+  std::call_once(onces[dev], [&rc] {
+    cudaError_t e = cudaSuccess;
+#define SETCA(HD, KT)                                                                       \
+  if (e == cudaSuccess)                                                                    \
+  e = cudaFuncSetAttribute(k_chunk_attention<HD, KT>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
+                           chunk_smem_bytes(HD, (int)sizeof(KT)))
+    SETCA(32, float);
+    SETCA(64, float);
+    SETCA(128, float);
+    SETCA(32, __half);
+    SETCA(64, __half);
+    SETCA(128, __half);
+#undef SETCA
+    rc = e == cudaSuccess ? L3G_OK
+                          : l3g_fail(L3G_E_CUDA, "chunk attention attributes: %s",
+                                     cudaGetErrorString(e));
+  });
+  return rc ? l3g_fail(L3G_E_CUDA, "chunk attention set-up failed on device %d", dev) : L3G_OK;
+}
 
 extern "C" void l3g_chunk_attn_free(l3g_chunk_attn* h) {
   if (!h) return;
   DeviceScope scope(h->device);
-  if (h->d_res) cudaFree(h->d_res);
+  void* d[] = {h->d_res, h->part_o, h->part_ml, h->split};
+  for (void* p : d)
+    if (p) cudaFree(p);
   delete h;
 }
 
@@ -60,6 +95,7 @@ extern "C" int l3g_chunk_attn_new(int32_t n_heads, int32_t n_heads_kv, int32_t h
   int dev = device;
   if (dev < 0) CUDA_TRY(cudaGetDevice(&dev));
   ON_DEVICE(dev);
+  if (int rc = chunk_setup()) return rc;
   auto* h = new l3g_chunk_attn();
   h->device = dev;
   h->nsm = sm_count(dev);
@@ -69,6 +105,10 @@ extern "C" int l3g_chunk_attn_new(int32_t n_heads, int32_t n_heads_kv, int32_t h
   h->kv_f16 = kv_dtype == L3G_KV_F16;
   cudaError_t e = cudaMalloc(&h->d_res, sizeof(Result));
   if (e == cudaSuccess) e = cudaMemset(h->d_res, 0, sizeof(Result));
+  const size_t rows = (size_t)2 * h->nsm * CHUNK_BM;  // two pieces per CTA
+  if (e == cudaSuccess) e = cudaMalloc(&h->part_o, rows * head_dim * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&h->part_ml, rows * 2 * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&h->split, (size_t)h->nsm * 8 * 4);
   if (e != cudaSuccess) {
     l3g_chunk_attn_free(h);
     return l3g_fail(L3G_E_CUDA, "chunk attention: %s", cudaGetErrorString(e));
@@ -79,9 +119,9 @@ extern "C" int l3g_chunk_attn_new(int32_t n_heads, int32_t n_heads_kv, int32_t h
 
 template <int HD, typename KT>
 static cudaError_t launch_chunk(const l3g_chunk_attn* h, const ChunkArgs& a, cudaStream_t st) {
-  const long long blocks = ((long long)a.total_q * a.heads + 7) / 8;
-  k_chunk_simple<HD, KT>
-      <<<dim3((unsigned)std::min<long long>(blocks, 8LL * h->nsm), a.n_seqs), 256, 0, st>>>(a);
+  k_chunk_attention<HD, KT>
+      <<<h->nsm, CHUNK_THREADS, chunk_smem_bytes(HD, (int)sizeof(KT)), st>>>(a);
+  k_chunk_merge<HD><<<dim3(h->nsm, 8), 256, 0, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -112,11 +152,14 @@ extern "C" int l3g_chunk_attn_run(l3g_chunk_attn* h, const l3g_chunk_seq* seqs, 
   a.out = out;
   a.ldo = ldo;
   a.layer = layer;
-  a.heads = h->heads;
   a.hkv = h->hkv;
   a.group = h->heads / h->hkv;
-  a.scale = scale > 0.0f ? scale : (float)(1.0 / sqrt((double)h->hd));
+  a.scale = (float)((scale > 0.0f ? (double)scale : 1.0 / sqrt((double)h->hd)) * M_LOG2E);
   a.res = h->d_res;
+  a.part_o = h->part_o;
+  a.part_ml = h->part_ml;
+  a.split = h->split;
+  a.wait_ns = WAIT_TIMEOUT_NS;
   const cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
   if (h->kv_f16)

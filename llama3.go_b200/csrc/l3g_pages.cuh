@@ -10,7 +10,7 @@ static __global__ void k_copy_pages(const uint8_t* sp, int n_src, uint8_t* dp, i
   for (int i = blockIdx.y; i < n; i += gridDim.y) {
     const int s = src[i], d = dst[i], r = rows ? rows[i] : KV_PAGE;
     if (s < 0 || s >= n_src || d < 0 || d >= n_dst || r < 0 || r > KV_PAGE) {
-      if (status && threadIdx.x == 0 && blockIdx.x == 0 && atomicCAS(status, 0, ERR_PAGE) == 0)
+      if (status && threadIdx.x == 0 && blockIdx.x == 0 && atomicCAS(status, 0, (int)ERR_PAGE) == 0)
         atomicExch(status + 1, i);
       continue;
     }

@@ -1,0 +1,153 @@
+// Host build of the serving operators' kernels (chunk attention, log
+// probabilities, page copies) under the SIMT emulator, with a C entry point
+// each for the CPU tests (ctypes).  Test infrastructure.
+#include "simt.h"
+
+#define execute_mma execute_mma_i8
+#include "simt_tcgen05.h"
+#undef execute_mma
+
+namespace simt {
+// kind::f16 with A in tensor memory: D[m][n] (+)= sum_k A[m][k] B[n][k], K = 16
+inline void execute_mma(const TensorOp& op) {
+  Block* b = op.blk;
+  const uint32_t id = op.idesc;
+  if (((id >> 4) & 3u) != 1u) fail("tcgen05.mma kind::f16: accumulator type is not f32");
+  if (((id >> 7) & 7u) || ((id >> 10) & 7u)) fail("tcgen05.mma kind::f16: operands are not f16");
+  if ((id >> 15) & 1u) fail("tcgen05.mma: A in tensor memory is K-major");
+  const bool mn_major = (id >> 16) & 1u;
+  const int M = (int)((id >> 24) & 0x1Fu) << 4, N = (int)((id >> 17) & 0x3Fu) << 3;
+  if (M != 128) fail("tcgen05.mma cta_group::1: only M = 128 is modelled");
+  if (N < 16 || N > 256 || N % 16) fail("tcgen05.mma: N must be a multiple of 16 in [16, 256]");
+  const SmemDesc B = decode_desc(op.bdesc);
+  const uint32_t a_col = (uint32_t)op.adesc & 0xFFFFu, d_col = op.d_tmem & 0xFFFFu;
+  if (((uint32_t)op.adesc >> 16) || (op.d_tmem >> 16)) fail("tcgen05.mma: M = 128 starts at lane 0");
+  auto used = [&](uint32_t c0, uint32_t n) {
+    if (c0 + n > 512) fail("tcgen05.mma past the last column");
+    for (uint32_t u = c0 / 32; u <= (c0 + n - 1) / 32; ++u)
+      if (!(b->tmem_used >> u & 1u)) fail("tcgen05.mma of tensor memory that is not allocated");
+  };
+  used(a_col, 8);
+  used(d_col, (uint32_t)N);
+  auto half_at = [](const uint8_t* p) {
+    uint16_t u;
+    memcpy(&u, p, 2);
+    __half_raw r;
+    r.x = u;
+    return __half2float(__half(r));
+  };
+  std::vector<float> bv((size_t)N * 16);
+  for (int n = 0; n < N; ++n)
+    for (int k = 0; k < 16; ++k) {
+      // K-major: 8 rows x 16 bytes per core matrix, rows of cores SBO apart, the
+      // two K halves LBO; MN-major: 8 K x 8 N, N groups SBO apart, K groups LBO
+      const size_t off = mn_major ? B.start + (size_t)(n / 8) * B.sbo + (size_t)(k / 8) * B.lbo +
+                                        (size_t)(k % 8) * 16 + (size_t)(n % 8) * 2
+                                  : B.start + (size_t)(n / 8) * B.sbo + (size_t)(k / 8) * B.lbo +
+                                        (size_t)(n % 8) * 16 + (size_t)(k % 8) * 2;
+      if (off + 2 > b->smem_bytes) fail("tcgen05.mma operand outside shared memory");
+      bv[(size_t)n * 16 + k] = half_at(b->smem + off);
+    }
+  for (int m = 0; m < M; ++m) {
+    float av[16];
+    for (int k = 0; k < 16; ++k)
+      av[k] = half_at(reinterpret_cast<const uint8_t*>(&b->tmem[(size_t)m * 512 + a_col]) + 2 * k);
+    for (int n = 0; n < N; ++n) {
+      float* cell = reinterpret_cast<float*>(&b->tmem[(size_t)m * 512 + d_col + n]);
+      float s = op.accumulate ? *cell : 0.0f;
+      for (int k = 0; k < 16; ++k) s += av[k] * bv[(size_t)n * 16 + k];
+      *cell = s;
+    }
+  }
+}
+}  // namespace simt
+
+#include "l3g.h"
+
+#define L3G_PTX_HEADER "simt_l3g_ptx.h"
+#include "l3g_kernels.cuh"
+
+namespace l3g {
+#include "simt_tc16.h"
+
+#include "l3g_chunk_attn.cuh"
+
+
+#include "l3g_pages.cuh"
+}  // namespace l3g
+
+namespace {
+std::string g_err;
+template <typename F>
+int guarded_call(F&& f) {
+  try {
+    f();
+    return 0;
+  } catch (const std::exception& e) {
+    g_err = e.what();
+    return -1;
+  }
+}
+template <int HD, typename KT>
+void run_chunk(const l3g::ChunkArgs& a, int grid) {
+  simt::launch(dim3(grid), dim3(l3g::CHUNK_THREADS), l3g::chunk_smem_bytes(HD, (int)sizeof(KT)),
+               [&] { l3g::k_chunk_attention<HD, KT>(a); });
+  simt::launch(dim3(grid, 8), dim3(256), 0, [&] { l3g::k_chunk_merge<HD>(a); }, true);
+}
+}  // namespace
+
+extern "C" {
+const char* emu_error() { return g_err.c_str(); }
+void emu_schedule(int randomize, unsigned long long seed, int max_copy_delay) {
+  simt::rt().randomize = randomize != 0;
+  simt::rt().rng.seed(seed);
+  simt::rt().max_copy_delay = max_copy_delay;
+}
+void* emu_malloc(unsigned long long bytes) {
+  void* p = nullptr;
+  guarded_call([&] { p = simt::dmalloc(bytes); });
+  return p;
+}
+void emu_free(void* p) { guarded_call([&] { simt::dfree(p); }); }
+
+// Chunk attention on a grid of `grid` CTAs; every pointer from emu_malloc.
+int emu_chunk_attention(const void* seqs, int n_seqs, int total_q, const float* q, long long ldq,
+                        float* out, long long ldo, int layer, int heads, int hkv, int hd,
+                        int kv_f16, float scale, int grid, int* err, int* where) {
+  std::vector<void*> scratch;
+  auto dm = [&](size_t bytes) {
+    void* p = simt::dmalloc(bytes);
+    scratch.push_back(p);
+    return p;
+  };
+  const int rc = guarded_call([&] {
+    l3g::ChunkArgs a{};
+    a.seqs = static_cast<const l3g_chunk_seq*>(seqs);
+    a.n_seqs = n_seqs;
+    a.total_q = total_q;
+    a.q = q;
+    a.ldq = ldq;
+    a.out = out;
+    a.ldo = ldo;
+    a.layer = layer;
+    a.hkv = hkv;
+    a.group = heads / hkv;
+    a.scale = (float)(scale * M_LOG2E);
+    a.part_o = static_cast<float*>(dm((size_t)2 * grid * 128 * hd * 4));
+    a.part_ml = static_cast<float*>(dm((size_t)2 * grid * 128 * 2 * 4));
+    a.split = static_cast<int*>(dm((size_t)grid * 8 * 4));
+    a.res = static_cast<l3g::Result*>(dm(sizeof(l3g::Result)));
+    a.wait_ns = 1ull << 60;
+    if (hd == 32 && kv_f16) run_chunk<32, __half>(a, grid);
+    else if (hd == 32) run_chunk<32, float>(a, grid);
+    else if (hd == 64 && kv_f16) run_chunk<64, __half>(a, grid);
+    else if (hd == 64) run_chunk<64, float>(a, grid);
+    else if (kv_f16) run_chunk<128, __half>(a, grid);
+    else run_chunk<128, float>(a, grid);
+    *err = a.res->err;
+    *where = a.res->where;
+  });
+  for (void* p : scratch) simt::dfree(p);
+  return rc;
+}
+}
