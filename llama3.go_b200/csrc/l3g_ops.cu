@@ -1,5 +1,7 @@
 // The serving operators: attention of token chunks over paged caches, log
 // probabilities, page copies.
+#include <cuda.h>
+
 #include "l3g_rt.h"
 
 namespace l3g {
@@ -41,7 +43,36 @@ struct l3g_chunk_attn {
   float* part_o = nullptr;   // pieces of row tiles that several CTAs share
   float* part_ml = nullptr;
   int* split = nullptr;
+  uint8_t* maps = nullptr;   // the loaders' tensor maps
+  CUtensorMap map;           // what they are made from
 };
+
+// The tensor map of a pool's rows in boxes of one panel: the base address is a
+// placeholder that the kernel replaces, and rows are checked by page id there.
+static int chunk_map(l3g_chunk_attn* h) {
+  typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                             const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                             CUtensorMapFloatOOBfill);
+  void* fn = nullptr;
+  cudaDriverEntryPointQueryResult found;
+  CUDA_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000,
+                                            cudaEnableDefault, &found));
+  if (!fn || found != cudaDriverEntryPointSuccess)
+    return l3g_fail(L3G_E_CUDA, "chunk attention: no cuTensorMapEncodeTiled in the driver");
+  const int es = h->kv_f16 ? 2 : 4;
+  const cuuint64_t dims[2] = {(cuuint64_t)2 * h->hd, 0x7fffffffull};
+  const cuuint64_t strides[1] = {(cuuint64_t)2 * h->hd * es};
+  const cuuint32_t box[2] = {(cuuint32_t)chunk_box_cols(h->hd, es), (cuuint32_t)chunk_bn(es)};
+  const cuuint32_t step[2] = {1, 1};
+  const CUresult r = reinterpret_cast<Encode>(fn)(
+      &h->map, es == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2,
+      h->part_o, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      chunk_row_bytes(h->hd, es) == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return l3g_fail(L3G_E_CUDA, "chunk attention: tensor map, error %d", (int)r);
+  return L3G_OK;
+}
 
 // Kernel attributes, once per device, with that device current.
 static int chunk_setup() {
@@ -74,7 +105,7 @@ static int chunk_setup() {
 extern "C" void l3g_chunk_attn_free(l3g_chunk_attn* h) {
   if (!h) return;
   DeviceScope scope(h->device);
-  void* d[] = {h->d_res, h->part_o, h->part_ml, h->split};
+  void* d[] = {h->d_res, h->part_o, h->part_ml, h->split, h->maps};
   for (void* p : d)
     if (p) cudaFree(p);
   delete h;
@@ -109,9 +140,14 @@ extern "C" int l3g_chunk_attn_new(int32_t n_heads, int32_t n_heads_kv, int32_t h
   if (e == cudaSuccess) e = cudaMalloc(&h->part_o, rows * head_dim * 4);
   if (e == cudaSuccess) e = cudaMalloc(&h->part_ml, rows * 2 * 4);
   if (e == cudaSuccess) e = cudaMalloc(&h->split, (size_t)h->nsm * 8 * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&h->maps, (size_t)h->nsm * CHUNK_LOAD * 128);
   if (e != cudaSuccess) {
     l3g_chunk_attn_free(h);
     return l3g_fail(L3G_E_CUDA, "chunk attention: %s", cudaGetErrorString(e));
+  }
+  if (int rc = chunk_map(h)) {
+    l3g_chunk_attn_free(h);
+    return rc;
   }
   *out = h;
   return L3G_OK;
@@ -159,6 +195,8 @@ extern "C" int l3g_chunk_attn_run(l3g_chunk_attn* h, const l3g_chunk_seq* seqs, 
   a.part_o = h->part_o;
   a.part_ml = h->part_ml;
   a.split = h->split;
+  a.maps = h->maps;
+  a.map = h->map;
   a.wait_ns = WAIT_TIMEOUT_NS;
   const cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;

@@ -3,6 +3,8 @@
 // each for the CPU tests (ctypes).  Test infrastructure.
 #include "simt.h"
 
+#include <cuda.h>
+
 #define execute_mma execute_mma_i8
 #include "simt_tcgen05.h"
 #undef execute_mma
@@ -19,7 +21,10 @@ inline void execute_mma(const TensorOp& op) {
   const int M = (int)((id >> 24) & 0x1Fu) << 4, N = (int)((id >> 17) & 0x3Fu) << 3;
   if (M != 128) fail("tcgen05.mma cta_group::1: only M = 128 is modelled");
   if (N < 16 || N > 256 || N % 16) fail("tcgen05.mma: N must be a multiple of 16 in [16, 256]");
-  const SmemDesc B = decode_desc(op.bdesc);
+  const uint32_t mode = (uint32_t)(op.bdesc >> 61) & 7u;  // swizzle: 2 128-byte, 4 64-byte rows
+  if (mode != 2 && mode != 4) fail("tcgen05 matrix descriptor: swizzle mode not modelled");
+  const uint32_t rb = mode == 2 ? 128 : 64;
+  const SmemDesc B = decode_desc(op.bdesc & ~(7ull << 61));
   const uint32_t a_col = (uint32_t)op.adesc & 0xFFFFu, d_col = op.d_tmem & 0xFFFFu;
   if (((uint32_t)op.adesc >> 16) || (op.d_tmem >> 16)) fail("tcgen05.mma: M = 128 starts at lane 0");
   auto used = [&](uint32_t c0, uint32_t n) {
@@ -39,12 +44,11 @@ inline void execute_mma(const TensorOp& op) {
   std::vector<float> bv((size_t)N * 16);
   for (int n = 0; n < N; ++n)
     for (int k = 0; k < 16; ++k) {
-      // K-major: 8 rows x 16 bytes per core matrix, rows of cores SBO apart, the
-      // two K halves LBO; MN-major: 8 K x 8 N, N groups SBO apart, K groups LBO
-      const size_t off = mn_major ? B.start + (size_t)(n / 8) * B.sbo + (size_t)(k / 8) * B.lbo +
-                                        (size_t)(k % 8) * 16 + (size_t)(n % 8) * 2
-                                  : B.start + (size_t)(n / 8) * B.sbo + (size_t)(k / 8) * B.lbo +
-                                        (size_t)(n % 8) * 16 + (size_t)(k % 8) * 2;
+      // 8 rows (K-major: N; MN-major: K) of rb bytes are SBO apart; N beyond a
+      // row (MN-major) is LBO away; pieces move by the address bits above them
+      const size_t row = mn_major ? k : n, col = (mn_major ? n : k) * 2;
+      const size_t lin = B.start + row / 8 * B.sbo + row % 8 * rb + col / rb * B.lbo + col % rb;
+      const size_t off = lin ^ ((lin >> 7 & (rb == 128 ? 7 : 3)) << 4);
       if (off + 2 > b->smem_bytes) fail("tcgen05.mma operand outside shared memory");
       bv[(size_t)n * 16 + k] = half_at(b->smem + off);
     }
@@ -136,6 +140,12 @@ int emu_chunk_attention(const void* seqs, int n_seqs, int total_q, const float* 
     a.part_o = static_cast<float*>(dm((size_t)2 * grid * 128 * hd * 4));
     a.part_ml = static_cast<float*>(dm((size_t)2 * grid * 128 * 2 * 4));
     a.split = static_cast<int*>(dm((size_t)grid * 8 * 4));
+    a.maps = static_cast<uint8_t*>(dm((size_t)grid * l3g::CHUNK_LOAD * 128));
+    {
+      const int es = kv_f16 ? 2 : 4;
+      l3g::EmuMap m{nullptr, 2 * hd * es, l3g::chunk_row_bytes(hd, es), l3g::chunk_bn(es), es};
+      memcpy(&a.map, &m, sizeof m);
+    }
     a.res = static_cast<l3g::Result*>(dm(sizeof(l3g::Result)));
     a.wait_ns = 1ull << 60;
     if (hd == 32 && kv_f16) run_chunk<32, __half>(a, grid);
