@@ -737,31 +737,43 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           corr = m == -INFINITY ? 0.0f : ex2(m - mu);
           m = mn;
           const float off = 13.0f - mu;
-          float sum = 0.0f, sum2 = 0.0f;
+          const unsigned long long ks2 = pk2(ks, ks), off2 = pk2(off, off);
+          const unsigned long long neg2 = pk2(-1.0f, -1.0f);
+          unsigned long long sum = 0ull, sum2 = 0ull;  // pairs of fp32
 #pragma unroll 1
-          for (int h = 0; h < BN / 16; ++h) {
-            uint32_t v[16];
-            tmem_ld16(t_s + h * 16, v);
+          for (int h = 0; h < BN; h += 32) {
+            uint32_t v[32];
+            tmem_ld32(t_s + h, v);
             tmem_wait_ld();
-            uint32_t ph[8], pl[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float x = ex2(fmaf(__uint_as_float(v[2 * i]), ks, off));
-              float y = ex2(fmaf(__uint_as_float(v[2 * i + 1]), ks, off));
-              if (!whole) {
-                if (h * 16 + 2 * i >= seen) x = 0.0f;
-                if (h * 16 + 2 * i + 1 >= seen) y = 0.0f;
+            for (int g = 0; g < 32; g += 16) {
+              uint32_t ph[8], pl[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int e = g + 2 * i;
+                const float2 t = upk2(
+                    fma2(pk2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), ks2, off2));
+                float x = ex2(t.x), y = ex2(t.y);
+                if (!whole) {
+                  if (h + e >= seen) x = 0.0f;
+                  if (h + e + 1 >= seen) y = 0.0f;
+                }
+                const unsigned long long p2 = pk2(x, y);
+                if (i & 1)
+                  sum2 = add2(sum2, p2);
+                else
+                  sum = add2(sum, p2);
+                ph[i] = pack_h2(x, y);
+                const float2 b = unpack_h2(ph[i]);
+                const float2 r = upk2(fma2(pk2(b.x, b.y), neg2, p2));
+                pl[i] = pack_h2(r.x, r.y);
               }
-              sum += x;
-              sum2 += y;
-              ph[i] = pack_h2(x, y);
-              const float2 b = unpack_h2(ph[i]);
-              pl[i] = pack_h2(x - b.x, y - b.y);
+              tmem_st8(t_s + h + g, ph);
+              tmem_st8(t_s + h + g + 8, pl);
             }
-            tmem_st8(t_s + h * 16, ph);
-            tmem_st8(t_s + h * 16 + 8, pl);
           }
-          l = fmaf(l, corr, sum + sum2);
+          const float2 total = upk2(add2(sum, sum2));
+          l = fmaf(l, corr, total.x + total.y);
           tmem_wait_st();
         }
         tc_fence_before();
