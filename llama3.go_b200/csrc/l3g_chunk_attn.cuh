@@ -52,6 +52,14 @@ struct ChunkArgs {
   CUtensorMap map;
 };
 
+// (see chunk_open)
+struct ChunkCursor {
+  long long pos, unit;  // next tile, first tile of its row tile
+  int s, kvh, rt, seg;
+  l3g_chunk_seq q;      // the sequence's descriptor
+  int nk, j0, j1;
+};
+
 struct ChunkSmem {
   uint8_t map[CHUNK_LOAD][128];  // (at the start: 128-byte aligned)
   uint64_t full[CHUNK_LOAD], empty[CHUNK_LOAD], raw[CHUNK_LOAD];  // K / V slots
@@ -65,10 +73,11 @@ struct ChunkSmem {
   int s0, kvh0, rt0, per;
   int bad[16];                   // segment + 1 whose pages are out of bounds
   float scale[32];               // f32 caches: 2^e of the items' tiles, item & 31
+  ChunkCursor cur[CHUNK_SOFT];   // the softmax warps' cursors, out of their registers
   float ml[2][CHUNK_BM][2];      // the groups' statistics
   long long pre[L3G_CHUNK_SEQS_MAX + 1];  // tiles before each sequence
 };
-constexpr int CHUNK_HEAD = 12288;
+constexpr int CHUNK_HEAD = 14 * 1024;
 static_assert(sizeof(ChunkSmem) <= CHUNK_HEAD, "chunk attention smem head");
 constexpr int CHUNK_TBUF = 32 * 33 * 4;  // a softmax warp's transposition buffer
 __host__ __device__ constexpr int chunk_slot_bytes(int hd, int es) {
@@ -103,14 +112,15 @@ __host__ __device__ constexpr int chunk_smem_bytes(int hd, int es) {
 }
 
 // Bounded wait as mbar_wait, for waits that are on the critical path many
-// times: the timer, which takes longer to read than most of the waits, is
-// looked at every 256th try.
+// times: the thread is suspended by the hardware (polling warps would take
+// issue slots from the others), 20 us a try, and the timer, which takes longer
+// to read than most of the waits, is looked at every 16th try.
 __device__ __forceinline__ bool chunk_wait(uint64_t* b, uint32_t parity, ChunkSmem* sh,
                                            const ChunkArgs& a, int where) {
   uint64_t t0 = 0;
-  for (int i = 0; !mbar_test(b, parity); ++i) {
+  for (int i = 0; !mbar_try_wait(b, parity, 20000); ++i) {
     if (*(volatile int*)&sh->abort_flag) return false;
-    if ((i & 255) == 255) {
+    if ((i & 15) == 15) {
       const uint64_t t = gtime();
       if (t0 == 0) t0 = t;
       if (t - t0 > a.wait_ns) {
@@ -142,12 +152,6 @@ __device__ __forceinline__ int chunk_tiles(const l3g_chunk_seq& s, int tt, int r
 // equal ranges; a row tile whose keys several CTAs hold is joined by
 // k_chunk_merge.  A cursor walks a CTA's range in segments, each the key tiles
 // [j0, j1) of one row tile.
-struct ChunkCursor {
-  long long pos, unit;  // next tile, first tile of its row tile
-  int s, kvh, rt, seg;
-  l3g_chunk_seq q;      // the sequence's descriptor
-  int nk, j0, j1;
-};
 template <int BN>
 __device__ __forceinline__ void chunk_open(const ChunkArgs& a, ChunkCursor& c, long long end) {
   c.nk = chunk_tiles<BN>(c.q, CHUNK_BM / a.group, c.rt);
@@ -284,6 +288,7 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
 __device__ __forceinline__ float2 unpack_h2(uint32_t u) {
   return __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 // 2^e as a float, e in [-126, 127]
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 // the exponent of the largest magnitude m, limited so that pow2i takes the
@@ -350,8 +355,6 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
-  ChunkCursor c;
-  bool more = chunk_first<BN>(a, sh, c);
 
   // two warpgroups give 64 of their 128 registers a thread to the other two
   if (warp >= CHUNK_SOFT) {
@@ -369,6 +372,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     int it = lw;                  // this warp's next item
     int it0 = 0;                  // the segment's first
     bool ok = lw < NS;
+    ChunkCursor c;
+    bool more = chunk_first<BN>(a, sh, c);
     for (; more && ok; more = chunk_next<BN>(a, sh, c)) {
       const int n = c.j1 - c.j0;
       const int* pages = c.q.pages + ((size_t)a.layer * a.hkv + c.kvh) * c.q.pps;
@@ -504,6 +509,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     int it = 0;
     // tiles of group 0 and 1 so far, issued to S and to O, over all segments
     int s0 = 0, s1 = 0, o0 = 0, o1 = 0, last = -1;
+    ChunkCursor c;
+    bool more = chunk_first<BN>(a, sh, c);
     bool ok = true, any = false;
     // the whole warp walks the loop, one lane issues
     auto wait = [&](uint64_t* b, int phase, int site) {
@@ -610,19 +617,23 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     int theirs = 0;  // ... of the other group
     bool ok = true;
     if (threadIdx.x == 0) a.split[blockIdx.x * 8] = 0;
-    for (; more && ok; more = chunk_next<BN>(a, sh, c)) {
+    ChunkCursor& c = sh->cur[warp];
+    bool more = false;
+    if (lane == 0) more = chunk_first<BN>(a, sh, c);
+    for (;;) {
+      if (!__shfl_sync(0xffffffffu, more, 0)) break;
+      __syncwarp();
       const int n = c.j1 - c.j0;
       const int ntok = min(tt, c.q.n_q - c.rt * tt);
       const int live_rows = ntok * a.group;
       const bool warp_live = (warp & 3) * 32 < live_rows;
       const bool live = row < live_rows;
+      const int seg = c.seg;
       // keys this row sees in all
       const int see = live ? c.q.kv_len - c.q.n_q + c.rt * tt + row / a.group + 1 : 0;
-      const long long row0 = (long long)c.q.q0 + c.rt * tt;
-      const float* qrow = a.q + (row0 + row / a.group) * a.ldq +
-                          (size_t)(c.kvh * a.group + row % a.group) * HD;
       float sc = 0.0f;
       if (warp_live) {
+        const long long row0 = (long long)c.q.q0 + c.rt * tt;
         // eight lanes read a row, four rows at a time, all in flight at once;
         // their hi (group 0) or lo (group 1) terms are turned in shared memory,
         // 64 dims at a time, to one row per lane
@@ -691,45 +702,57 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 
       unsigned long long o2[HD / 2];  // the output, dims 2 i and 2 i + 1
       float m = -INFINITY, l = 0.0f;
+      const int seen0 = see - c.j0 * BN;  // keys from the segment's first on that the row sees
 #pragma unroll
       for (int d = 0; d < HD / 2; ++d) o2[d] = 0ull;
       for (int j = w; j < n; j += 2, ++done) {
         ok = __all_sync(0xffffffffu, chunk_wait(&sh->s_full[w], done & 1, sh, a, 49));
         if (!ok) break;
         tc_fence_after();
-        const int kb = (c.j0 + j) * BN;
-        const int seen = see - kb < 0 ? 0 : see - kb > BN ? BN : see - kb;
+        const int seen = min(max(seen0 - j * BN, 0), BN);
         float corr = 1.0f, vs = 1.0f;
         const bool whole = __all_sync(0xffffffffu, seen == BN || !live);
         // the tile's K and V among the loaded items (a loader is at most NS + 4
         // items ahead of the softmax groups)
-        const int item0 = 2 * (int)(c.unit + c.j0 - sh->begin);
+        const int item0 = ES == 4 ? 2 * (int)(c.unit + c.j0 - sh->begin) : 0;
         const int item_k = item0 + (j == 0 ? 0 : 2 * j - 1);
         const int item_v = item0 + (j == n - 1 ? 2 * n - 1 : 2 * j + 2);
         if (warp_live) {
           float ks = sc;
           if constexpr (ES == 4) ks *= *(volatile float*)&sh->scale[item_k & 31];
+          // both passes over the scores load 16 columns ahead
           float mx = -INFINITY;
+          uint32_t v0[16], v1[16];
+          tmem_ld16(t_s, v0);
+          tmem_wait_ld16(v0);
           if (whole) {
+            float m2 = -INFINITY;
 #pragma unroll 1
             for (int h = 0; h < BN; h += 32) {
-              uint32_t v[32];
-              tmem_ld32(t_s + h, v);
-              tmem_wait_ld();
-              float m2[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
+              tmem_ld16(t_s + h + 16, v1);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) m2[i & 3] = fmaxf(m2[i & 3], __uint_as_float(v[i]));
-              mx = fmaxf(fmaxf(m2[0], m2[1]), fmaxf(m2[2], m2[3]));
+              for (int i = 0; i < 16; i += 4) {
+                mx = max3(mx, __uint_as_float(v0[i]), __uint_as_float(v0[i + 1]));
+                m2 = max3(m2, __uint_as_float(v0[i + 2]), __uint_as_float(v0[i + 3]));
+              }
+              tmem_wait_ld16(v1);
+              tmem_ld16(t_s + ((h + 32) & (BN - 1)), v0);  // at the end: the first again
+#pragma unroll
+              for (int i = 0; i < 16; i += 4) {
+                mx = max3(mx, __uint_as_float(v1[i]), __uint_as_float(v1[i + 1]));
+                m2 = max3(m2, __uint_as_float(v1[i + 2]), __uint_as_float(v1[i + 3]));
+              }
+              tmem_wait_ld16(v0);
             }
+            mx = fmaxf(mx, m2);
           } else {
 #pragma unroll 1
             for (int h = 0; h < BN; h += 16) {
-              uint32_t v[16];
-              tmem_ld16(t_s + h, v);
-              tmem_wait_ld();
 #pragma unroll
               for (int i = 0; i < 16; ++i)
-                if (h + i < seen) mx = fmaxf(mx, __uint_as_float(v[i]));
+                if (h + i < seen) mx = fmaxf(mx, __uint_as_float(v0[i]));
+              tmem_ld16(t_s + ((h + 16) & (BN - 1)), v0);
+              tmem_wait_ld16(v0);
             }
           }
           const float mn = fmaxf(m, mx * ks);
@@ -740,37 +763,39 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           const unsigned long long ks2 = pk2(ks, ks), off2 = pk2(off, off);
           const unsigned long long neg2 = pk2(-1.0f, -1.0f);
           unsigned long long sum = 0ull, sum2 = 0ull;  // pairs of fp32
+          // weights of 16 keys from their scores v, stored over them
+          auto weigh = [&](const uint32_t* v, int h) {
+            uint32_t ph[8], pl[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float2 t = upk2(
+                  fma2(pk2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ks2, off2));
+              float x = ex2(t.x), y = ex2(t.y);
+              if (!whole) {
+                if (h + 2 * i >= seen) x = 0.0f;
+                if (h + 2 * i + 1 >= seen) y = 0.0f;
+              }
+              const unsigned long long p2 = pk2(x, y);
+              if (i & 1)
+                sum2 = add2(sum2, p2);
+              else
+                sum = add2(sum, p2);
+              ph[i] = pack_h2(x, y);
+              const float2 b = unpack_h2(ph[i]);
+              const float2 r = upk2(fma2(pk2(b.x, b.y), neg2, p2));
+              pl[i] = pack_h2(r.x, r.y);
+            }
+            tmem_st8(t_s + h, ph);
+            tmem_st8(t_s + h + 8, pl);
+          };
 #pragma unroll 1
           for (int h = 0; h < BN; h += 32) {
-            uint32_t v[32];
-            tmem_ld32(t_s + h, v);
-            tmem_wait_ld();
-#pragma unroll
-            for (int g = 0; g < 32; g += 16) {
-              uint32_t ph[8], pl[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int e = g + 2 * i;
-                const float2 t = upk2(
-                    fma2(pk2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), ks2, off2));
-                float x = ex2(t.x), y = ex2(t.y);
-                if (!whole) {
-                  if (h + e >= seen) x = 0.0f;
-                  if (h + e + 1 >= seen) y = 0.0f;
-                }
-                const unsigned long long p2 = pk2(x, y);
-                if (i & 1)
-                  sum2 = add2(sum2, p2);
-                else
-                  sum = add2(sum, p2);
-                ph[i] = pack_h2(x, y);
-                const float2 b = unpack_h2(ph[i]);
-                const float2 r = upk2(fma2(pk2(b.x, b.y), neg2, p2));
-                pl[i] = pack_h2(r.x, r.y);
-              }
-              tmem_st8(t_s + h + g, ph);
-              tmem_st8(t_s + h + g + 8, pl);
-            }
+            tmem_ld16(t_s + h + 16, v1);
+            weigh(v0, h);
+            tmem_wait_ld16(v1);
+            if (h + 32 < BN) tmem_ld16(t_s + h + 32, v0);
+            weigh(v1, h + 16);
+            tmem_wait_ld16(v0);
           }
           const float2 total = upk2(add2(sum, sum2));
           l = fmaf(l, corr, total.x + total.y);
@@ -798,6 +823,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             odd = odd && live && seen < BN;
           }
           if (__any_sync(0xffffffffu, odd)) {
+            const int kb = (c.j0 + j) * BN;
+            const float* qrow = a.q + ((long long)c.q.q0 + c.rt * tt + row / a.group) * a.ldq +
+                                (size_t)(c.kvh * a.group + row % a.group) * HD;
             int page = 0;
             if (seen > 0)
               page = c.q.pages[((size_t)a.layer * a.hkv + c.kvh) * c.q.pps + kb / KV_PAGE];
@@ -871,14 +899,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->xchg);
-      ok = __all_sync(0xffffffffu, chunk_wait(&sh->xchg, c.seg & 1, sh, a, 51));
+      ok = __all_sync(0xffffffffu, chunk_wait(&sh->xchg, seg & 1, sh, a, 51));
       if (!ok) break;
       tc_fence_after();
       const bool split = c.j0 > 0 || c.j1 < c.nk;
-      const bool bad = *(volatile int*)&sh->bad[c.seg & 15] == c.seg + 1;
+      const bool bad = *(volatile int*)&sh->bad[seg & 15] == seg + 1;
       // a piece that begins its row tile goes to the CTA's second place
       const size_t place = 2 * (size_t)blockIdx.x + (c.j0 == 0 ? 1 : 0);
       if (warp_live) {
+        const long long row0 = (long long)c.q.q0 + c.rt * tt;
         const float m2 = sh->ml[w ^ 1][row][0], l2 = sh->ml[w ^ 1][row][1];
         const float M = fmaxf(m, m2);
         const float f = m == -INFINITY ? 0.0f : ex2(m - M);
@@ -937,6 +966,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         d[3] = c.kvh;
         d[4] = c.rt;
       }
+      __syncwarp();
+      if (lane == 0) more = chunk_next<BN>(a, sh, c);
     }
   }
   cp_async_wait<0>();
