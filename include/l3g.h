@@ -511,7 +511,7 @@ void l3g_chunk_attn_free(l3g_chunk_attn *h);
  * head's tokens that see it, at least), and noted for l3g_chunk_attn_status.
  * A NaN or an infinity in K or V gives NaN in the rows that see it and touches
  * no other. */
-#define L3G_CHUNK_SEQS_MAX 1024
+#define L3G_CHUNK_SEQS_MAX 512
 int l3g_chunk_attn_run(l3g_chunk_attn *h, const l3g_chunk_seq *seqs,
                        int32_t n_seqs, int32_t total_q, const float *q,
                        int64_t ldq, float *out, int64_t ldo, int32_t layer,

@@ -23,9 +23,19 @@ constexpr int CHUNK_BM = 128;       // rows per tile: lanes of tensor memory
 // keys per tile (divides KV_PAGE): 128 of an f16 cache; 64 of an f32 cache,
 // whose tiles take twice the shared memory
 __host__ __device__ constexpr int chunk_bn(int es) { return es == 2 ? 128 : 64; }
-constexpr int CHUNK_SOFT = 8;       // softmax warps: two groups of four
-constexpr int CHUNK_LOAD = 7;       // loader warps
-constexpr int CHUNK_THREADS = 32 * (CHUNK_SOFT + CHUNK_LOAD + 1);
+// warps: 16 softmax (four groups of four: group g is team g & 1, key half
+// g >> 1), 4 output, 7 loaders, 1 that issues the products
+constexpr int CHUNK_SOFT = 16;
+constexpr int CHUNK_OUT = 4;
+constexpr int CHUNK_LOAD = 7;
+constexpr int CHUNK_WARP_OUT = CHUNK_SOFT;
+constexpr int CHUNK_WARP_LOAD = CHUNK_WARP_OUT + CHUNK_OUT;
+constexpr int CHUNK_WARP_MMA = CHUNK_WARP_LOAD + CHUNK_LOAD;
+constexpr int CHUNK_WARPS = CHUNK_WARP_MMA + 1;
+constexpr int CHUNK_THREADS = 32 * CHUNK_WARPS;
+// registers per thread after the split; the block has 72 x 896 = 504 x 128
+constexpr int CHUNK_R_SOFT = 64, CHUNK_R_OUT = 168, CHUNK_R_REST = 40;
+static_assert(4 * CHUNK_R_SOFT + CHUNK_R_OUT + 2 * CHUNK_R_REST <= 504, "register split");
 constexpr int CHUNK_MIN_KEYS = 256;  // keys a CTA takes at least
 __host__ __device__ constexpr int chunk_min_tiles(int bn) { return CHUNK_MIN_KEYS / bn; }
 // tensor-memory columns: scores / weights of the two groups (at most 128
@@ -63,8 +73,9 @@ struct ChunkCursor {
 struct ChunkSmem {
   uint8_t map[CHUNK_LOAD][128];  // (at the start: 128-byte aligned)
   uint64_t full[CHUNK_LOAD], empty[CHUNK_LOAD], raw[CHUNK_LOAD];  // K / V slots
-  uint64_t s_full[2], p_full[2], o_full[2], o_free[2];
-  uint64_t q_ready, xchg, drain;
+  uint64_t s_full[2], p_full[2], o_full;
+  uint64_t q_ready, l_full, e_done, drain;
+  uint64_t qx[4], mx[2][4];      // per quarter of the rows: its groups met
   uint32_t tmem_base;
   int abort_flag;
   int n_tiles_lo, pad;
@@ -73,24 +84,27 @@ struct ChunkSmem {
   int s0, kvh0, rt0, per;
   int bad[16];                   // segment + 1 whose pages are out of bounds
   float scale[32];               // f32 caches: 2^e of the items' tiles, item & 31
-  ChunkCursor cur[CHUNK_SOFT];   // the softmax warps' cursors, out of their registers
-  float ml[2][CHUNK_BM][2];      // the groups' statistics
+  ChunkCursor cur[CHUNK_WARPS];  // the warps' cursors, out of their registers
+  float qmax[4][CHUNK_BM];       // largest |q| of each group's dims
+  float gmax[2][2][2][CHUNK_BM]; // a tile's maxima [team][tile][key half]
+  float m_tile[4][CHUNK_BM];     // what a tile's weights are relative to
+  float m_team[2][CHUNK_BM], l_group[4][CHUNK_BM];  // a segment's statistics
   long long pre[L3G_CHUNK_SEQS_MAX + 1];  // tiles before each sequence
 };
-constexpr int CHUNK_HEAD = 14 * 1024;
+constexpr int CHUNK_HEAD = 20 * 1024;
 static_assert(sizeof(ChunkSmem) <= CHUNK_HEAD, "chunk attention smem head");
-constexpr int CHUNK_TBUF = 32 * 33 * 4;  // a softmax warp's transposition buffer
+constexpr int CHUNK_TBUF = 32 * 17 * 4;  // a softmax or output warp's transposition buffer
 __host__ __device__ constexpr int chunk_slot_bytes(int hd, int es) {
   return chunk_bn(es) * hd * es;  // f16: one operand tile; f32: its hi and lo tiles
 }
 // one slot per loader warp, as far as they fit
 __host__ __device__ constexpr int chunk_slots(int hd, int es) {
-  return (180 * 1024) / chunk_slot_bytes(hd, es) < CHUNK_LOAD
-             ? (180 * 1024) / chunk_slot_bytes(hd, es)
+  return (160 * 1024) / chunk_slot_bytes(hd, es) < CHUNK_LOAD
+             ? (160 * 1024) / chunk_slot_bytes(hd, es)
              : CHUNK_LOAD;
 }
 __host__ __device__ constexpr int chunk_ring_off() {
-  return (CHUNK_HEAD + CHUNK_SOFT * CHUNK_TBUF + 1023) / 1024 * 1024;
+  return (CHUNK_HEAD + (CHUNK_SOFT + CHUNK_OUT) * CHUNK_TBUF + 1023) / 1024 * 1024;
 }
 // Operand tiles in shared memory: panels of up to 64 dims, [key][row bytes] with
 // the 16-byte pieces of a row swizzled by the key (the tensor core's 128-byte
@@ -111,26 +125,26 @@ __host__ __device__ constexpr int chunk_smem_bytes(int hd, int es) {
   return chunk_ring_off() + chunk_slots(hd, es) * chunk_slot_bytes(hd, es);
 }
 
-// Bounded wait as mbar_wait, for waits that are on the critical path many
-// times: the thread is suspended by the hardware (polling warps would take
-// issue slots from the others), 20 us a try, and the timer, which takes longer
-// to read than most of the waits, is looked at every 16th try.
+// Bounded wait of a whole warp, for waits that are on the critical path many
+// times: no divergence, the warp suspended by the hardware (polling warps
+// would take issue slots from the others) for 20 us a try, and the timer, which
+// takes longer to read than most of the waits, looked at every 16th try.
 __device__ __forceinline__ bool chunk_wait(uint64_t* b, uint32_t parity, ChunkSmem* sh,
                                            const ChunkArgs& a, int where) {
   uint64_t t0 = 0;
-  for (int i = 0; !mbar_try_wait(b, parity, 20000); ++i) {
-    if (*(volatile int*)&sh->abort_flag) return false;
+  for (int i = 0;; ++i) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(b, parity, 20000))) return true;
+    if (__any_sync(0xffffffffu, *(volatile int*)&sh->abort_flag)) return false;
     if ((i & 15) == 15) {
       const uint64_t t = gtime();
       if (t0 == 0) t0 = t;
-      if (t - t0 > a.wait_ns) {
+      if (__any_sync(0xffffffffu, t - t0 > a.wait_ns)) {
         *(volatile int*)&sh->abort_flag = 1;
-        report(a.res, ERR_TIMEOUT, where);
+        if ((threadIdx.x & 31) == 0) report(a.res, ERR_TIMEOUT, where);
         return false;
       }
     }
   }
-  return true;
 }
 
 // Whether a descriptor stays inside its bounds (its pages are checked where
@@ -281,6 +295,14 @@ __device__ __forceinline__ void chunk_row_slow(const KT* rows, int n, const floa
   }
 }
 
+// N words to N columns of the warp's lanes of tensor memory
+template <int N>
+__device__ __forceinline__ void tmem_stn(uint32_t t, const uint32_t* v) {
+  if constexpr (N == 16) tmem_st16(t, v);
+  else if constexpr (N == 8) tmem_st8(t, v);
+  else tmem_st4(t, v);
+}
+
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -298,13 +320,16 @@ __device__ __forceinline__ int exp_of(float m) {
   return e < -100 ? -100 : e > 127 ? 127 : e;
 }
 
-// Roles: softmax groups 0 and 1 (warps 0-3 and 4-7; thread = row), taking the
-// segment's key tiles in turn, each with statistics and an output of its own,
-// joined at the segment's end; loader warps 8-14, which bring K and V tiles
-// into a ring of shared-memory slots in the order the products use them
-// (K0 K1 V0 K2 V1 ...); warp 15, whose lane 0 issues the products:
+// Roles.  One warp issues the products, in the order S0 S1 O0 S2 O1 ...:
 //   S = q K^T   A = q from tensor memory, B = K tile  [key][dim], K-major
 //   O = p V     A = p from tensor memory (over S), B = V tile [key][dim], MN-major
+// Seven loader warps bring the tiles into a ring of shared-memory slots in that
+// order.  Sixteen softmax warps turn scores into weights: two teams take the
+// tiles in turn (there are two S), a thread a row and half of the tile's keys;
+// each team has a running maximum of its own.  Four output warps, a thread a
+// row, add a tile's output, scaled to the maximum over both teams, to the
+// registers that hold the row's.  The tensor core waits for the weights of tile
+// j only after it has been given the scores of tile j + 1.
 // Either tile is panels of [key][dims], swizzled (chunk_piece).
 template <int HD, typename KT>
 __global__ void __launch_bounds__(CHUNK_THREADS, 1)
@@ -335,12 +360,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(&sh->s_full[w], 1);
-      mbar_init(&sh->p_full[w], 4);
-      mbar_init(&sh->o_full[w], 1);
-      mbar_init(&sh->o_free[w], 4);
+      mbar_init(&sh->p_full[w], CHUNK_SOFT / 2 + CHUNK_OUT);
+      for (int i = 0; i < 4; ++i) mbar_init(&sh->mx[w][i], 2);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&sh->qx[i], 4);
+    mbar_init(&sh->o_full, 1);
     mbar_init(&sh->q_ready, CHUNK_SOFT);
-    mbar_init(&sh->xchg, CHUNK_SOFT);
+    mbar_init(&sh->l_full, CHUNK_SOFT);
+    mbar_init(&sh->e_done, CHUNK_OUT);
     mbar_init(&sh->drain, 1);
     sh->abort_flag = 0;
     for (int i = 0; i < 16; ++i) sh->bad[i] = 0;
@@ -350,31 +377,49 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     __syncwarp();
     chunk_plan<BN>(a, sh, lane);
   }
-  if (warp == 15) tmem_alloc(&sh->tmem_base, CHUNK_T_COLS);
+  if (warp == CHUNK_WARP_MMA) tmem_alloc(&sh->tmem_base, CHUNK_T_COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
 
-  // two warpgroups give 64 of their 128 registers a thread to the other two
-  if (warp >= CHUNK_SOFT) {
-  regs_dec<64>();
-  if (warp < CHUNK_SOFT + CHUNK_LOAD) {
+  // every warp walks the CTA's segments with a cursor of its own
+  ChunkCursor& c = sh->cur[warp];
+  auto first = [&] {
+    bool more = false;
+    if (lane == 0) more = chunk_first<BN>(a, sh, c);
+    return __shfl_sync(0xffffffffu, more ? 1 : 0, 0) != 0;
+  };
+  auto next = [&] {
+    bool more = false;
+    __syncwarp();
+    if (lane == 0) more = chunk_next<BN>(a, sh, c);
+    return __shfl_sync(0xffffffffu, more ? 1 : 0, 0) != 0;
+  };
+  auto wait = [&](uint64_t* b, int phase, int site) {
+    return chunk_wait(b, phase & 1, sh, a, site);
+  };
+  const int quarter = warp & 3;          // softmax and output warps: their rows
+  const int row = quarter * 32 + lane;
+  const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
+  bool ok = true;
+
+  if (warp >= CHUNK_WARP_LOAD) {
+  regs_dec<CHUNK_R_REST>();
+  if (warp < CHUNK_WARP_MMA) {
     // ---- loaders ----------------------------------------------------------
     // Warp lw brings the items lw, lw + NS, ... whole into slot lw: a tile whose
     // keys all exist by tensor copies (one box per panel), the last, part-filled
     // one by 16-byte copies with zeros for the keys past the cache's end.
-    const int lw = warp - CHUNK_SOFT;
+    const int lw = warp - CHUNK_WARP_LOAD;
     const int kl = lane >> 3, cl = lane & 7;  // key and piece of the lane
     uint8_t* map = a.maps + ((size_t)blockIdx.x * CHUNK_LOAD + lw) * 128;
     const void* map_pool = nullptr;
     uint8_t* const dst = ring + (size_t)lw * SLOT;
     int it = lw;                  // this warp's next item
     int it0 = 0;                  // the segment's first
-    bool ok = lw < NS;
-    ChunkCursor c;
-    bool more = chunk_first<BN>(a, sh, c);
-    for (; more && ok; more = chunk_next<BN>(a, sh, c)) {
+    ok = lw < NS;
+    for (bool more = first(); more && ok; more = next()) {
       const int n = c.j1 - c.j0;
       const int* pages = c.q.pages + ((size_t)a.layer * a.hkv + c.kvh) * c.q.pps;
       for (; it < it0 + 2 * n; it += NS) {
@@ -398,7 +443,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         }
         const int use = it / NS;
         if (use > 0) {
-          ok = __all_sync(0xffffffffu, chunk_wait(&sh->empty[lw], (use - 1) & 1, sh, a, 40));
+          ok = chunk_wait(&sh->empty[lw], (use - 1) & 1, sh, a, 40);
           if (!ok) break;
         }
         // (after the wait: the slot's last copy, which used the map, is over)
@@ -436,7 +481,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           if (lane == 0) mbar_arrive(landed);
         }
         if constexpr (ES == 4) {
-          ok = __all_sync(0xffffffffu, chunk_wait(&sh->raw[lw], use & 1, sh, a, 41));
+          ok = chunk_wait(&sh->raw[lw], use & 1, sh, a, 41);
           if (!ok) break;
           // the tile's scale, from its largest finite magnitude
           float m = 0.0f;
@@ -506,29 +551,25 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     constexpr uint64_t DESC_K = gemm::smem_desc(0, 16, 8 * RB) | SWZ;
     constexpr uint64_t DESC_V = gemm::smem_desc(0, NEXT, 8 * RB) | SWZ;
     const uint32_t ring0 = smem_u32(ring) >> 4;
-    int it = 0;
-    // tiles of group 0 and 1 so far, issued to S and to O, over all segments
-    int s0 = 0, s1 = 0, o0 = 0, o1 = 0, last = -1;
-    ChunkCursor c;
-    bool more = chunk_first<BN>(a, sh, c);
-    bool ok = true, any = false;
-    // the whole warp walks the loop, one lane issues
-    auto wait = [&](uint64_t* b, int phase, int site) {
-      return __all_sync(0xffffffffu, chunk_wait(b, phase & 1, sh, a, site)) != 0;
-    };
-    for (; more && ok; more = chunk_next<BN>(a, sh, c)) {
+    // The whole warp walks the loop, one lane issues.  The tensor core takes
+    // new products only while it has few left, so what a batch needs is waited
+    // for as early as its order allows.
+    int it = 0;          // slots used
+    int ns = 0, no = 0;  // tiles so far, issued to S and to O
+    for (bool more = first(); more && ok; more = next()) {
       const int n = __shfl_sync(0xffffffffu, c.j1 - c.j0, 0);
       ok = wait(&sh->q_ready, c.seg, 42);
-      if (!ok) break;
-      tc_fence_after();
+      // at a segment's start every product so far is complete
+      if (ok && ns > 0) ok = wait(&sh->o_full, ns - 1, 44);
       for (int j = 0; j <= n && ok; ++j) {
+        const int slot = it % NS, slot2 = (it + 1) % NS;
+        ok = wait(&sh->full[slot], it / NS, 43);
+        if (ok && j >= 1 && j < n) ok = wait(&sh->full[slot2], (it + 1) / NS, 45);
         if (j < n) {
-          const int w = j & 1, slot = it % NS;
-          ok = wait(&sh->full[slot], it / NS, 43);
-          // the weights of the group's previous tile lie over S until its
-          // second product is complete
-          const int before = w ? s1 : s0;
-          if (ok && before > 0) ok = wait(&sh->o_full[w], before - 1, 44);
+          const int w = ns & 1;
+          // the weights of the tile before the last lie over S until their
+          // product is complete
+          if (ok && j > 1) ok = wait(&sh->o_full, ns - 2, 44);
           if (!ok) break;
           tc_fence_after();
           const uint32_t b0 = ring0 + (uint32_t)(slot * (SLOT >> 4)) + (uint32_t)DESC_K;
@@ -552,22 +593,16 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             mma_commit(&sh->empty[slot]);
           }
           __syncwarp();
-          any = true;
-          if (w)
-            ++s1;
-          else
-            ++s0;
+          ++ns;
           ++it;
         }
         if (j >= 1) {
-          const int w = (j - 1) & 1, slot = it % NS;
-          ok = wait(&sh->full[slot], it / NS, 45);
-          if (ok) ok = wait(&sh->p_full[w], w ? o1 : o0, 46);
-          // the output of the tile before, of group `last`, has been read
-          if (ok && last >= 0) ok = wait(&sh->o_free[last], (last ? o1 : o0) - 1, 47);
+          const int w = no & 1, vs = j < n ? slot2 : slot;
+          // the weights are there and the output of the tile before has been read
+          ok = wait(&sh->p_full[w], no >> 1, 46);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t b0 = ring0 + (uint32_t)(slot * (SLOT >> 4)) + (uint32_t)DESC_V;
+          const uint32_t b0 = ring0 + (uint32_t)(vs * (SLOT >> 4)) + (uint32_t)DESC_V;
           const uint32_t pw = tmem + CHUNK_T_S + w * BN;
           const uint32_t d = tmem + CHUNK_T_O;
           if (elect_one()) {
@@ -584,377 +619,162 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                   mma_f16_ts<true>(d, pa, bb + k * RB, (uint32_t)(DESC_V >> 32), IDESC_O);  // 16 keys
               }
             }
-            mma_commit(&sh->o_full[w]);
-            mma_commit(&sh->empty[slot]);
+            mma_commit(&sh->o_full);
+            mma_commit(&sh->empty[vs]);
           }
           __syncwarp();
-          if (w)
-            ++o1;
-          else
-            ++o0;
-          last = w;
+          ++no;
           ++it;
         }
       }
     }
-    if (any) {  // every product issued has completed before the memory goes
+    if (ns > 0) {  // every product issued has completed before the memory goes
       if (elect_one()) mma_commit(&sh->drain);
       int dummy = 0;
       mbar_wait(&sh->drain, 0, &dummy, a.res, 48, a.wait_ns);
     }
     __syncwarp();
   }
-  } else {
-    // ---- softmax groups -----------------------------------------------------
-    regs_inc<192>();
-    const int w = warp >> 2;             // group
-    const int row = threadIdx.x & 127;   // row = lane of tensor memory
-    const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t t_s = t_lane + CHUNK_T_S + w * BN, t_o = t_lane + CHUNK_T_O;
-    const uint32_t t_mine = t_o + w * (HD / 2), t_theirs = t_o + (w ^ 1) * (HD / 2);
-    float* tb = tbuf + warp * 32 * 33;
-    int done = 0;    // tiles of this group so far
-    int theirs = 0;  // ... of the other group
-    bool ok = true;
-    if (threadIdx.x == 0) a.split[blockIdx.x * 8] = 0;
-    ChunkCursor& c = sh->cur[warp];
-    bool more = false;
-    if (lane == 0) more = chunk_first<BN>(a, sh, c);
-    for (;;) {
-      if (!__shfl_sync(0xffffffffu, more, 0)) break;
-      __syncwarp();
-      const int n = c.j1 - c.j0;
-      const int ntok = min(tt, c.q.n_q - c.rt * tt);
-      const int live_rows = ntok * a.group;
-      const bool warp_live = (warp & 3) * 32 < live_rows;
-      const bool live = row < live_rows;
-      const int seg = c.seg;
-      // keys this row sees in all
-      const int see = live ? c.q.kv_len - c.q.n_q + c.rt * tt + row / a.group + 1 : 0;
-      float sc = 0.0f;
-      if (warp_live) {
-        const long long row0 = (long long)c.q.q0 + c.rt * tt;
-        // eight lanes read a row, four rows at a time, all in flight at once;
-        // their hi (group 0) or lo (group 1) terms are turned in shared memory,
-        // 64 dims at a time, to one row per lane
-        const int rl4 = lane >> 3, l8 = lane & 7;
-        float4 x[8][HD / 32];
-        float up[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = (warp & 3) * 32 + i * 4 + rl4;
-          const float* g = a.q + (row0 + r / a.group) * a.ldq +
-                           (size_t)(c.kvh * a.group + r % a.group) * HD + l8 * 4;
-#pragma unroll
-          for (int k = 0; k < HD / 32; ++k)
-            x[i][k] = r < live_rows ? *reinterpret_cast<const float4*>(g + k * 32)
-                                    : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float m4 = 0.0f;
-#pragma unroll
-          for (int k = 0; k < HD / 32; ++k)
-            m4 = fmaxf(fmaxf(fmaxf(m4, fabsf(x[i][k].x)), fmaxf(fabsf(x[i][k].y), fabsf(x[i][k].z))),
-                       fabsf(x[i][k].w));
-#pragma unroll
-          for (int o = 1; o < 8; o <<= 1) m4 = fmaxf(m4, __shfl_xor_sync(0xffffffffu, m4, o));
-          // the row's largest value lands in [2^10, 2^11); row i * 4 + k of the
-          // warp is lane i * 4 + k's
-          up[i] = pow2i(10 - exp_of(m4));
-          const float mine = __shfl_sync(0xffffffffu, up[i], (lane & 3) * 8);
-          if ((lane >> 2) == i) sc = a.scale / mine;
-        }
-        uint32_t* tw = reinterpret_cast<uint32_t*>(tb);
-        constexpr int QH = HD < 64 ? HD : 64;  // dims at a time
-#pragma unroll
-        for (int h = 0; h < HD; h += QH) {
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int k = 0; k < QH / 32; ++k) {
-              const float4 y = x[i][h / 32 + k];
-              uint32_t p0 = pack_h2(y.x * up[i], y.y * up[i]);
-              uint32_t p1 = pack_h2(y.z * up[i], y.w * up[i]);
-              if (w == 1) {
-                const float2 b0 = unpack_h2(p0), b1 = unpack_h2(p1);
-                p0 = pack_h2(fmaf(y.x, up[i], -b0.x), fmaf(y.y, up[i], -b0.y));
-                p1 = pack_h2(fmaf(y.z, up[i], -b1.x), fmaf(y.w, up[i], -b1.y));
-              }
-              tw[(i * 4 + rl4) * 33 + k * 16 + l8 * 2] = p0;
-              tw[(i * 4 + rl4) * 33 + k * 16 + l8 * 2 + 1] = p1;
-            }
-          __syncwarp();
-#pragma unroll
-          for (int e = 0; e < QH / 2; e += 16) {
-            uint32_t u[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) u[i] = tw[lane * 33 + e + i];
-            tmem_st16(t_lane + CHUNK_T_Q + w * (HD / 2) + h / 2 + e, u);
-          }
-        }
-        tmem_wait_st();
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->q_ready);
-
+  } else if (warp >= CHUNK_WARP_OUT) {
+    // ---- output -------------------------------------------------------------
+    regs_inc<CHUNK_R_OUT>();
+    const uint32_t t_o = t_lane + CHUNK_T_O;
+    float* tb = tbuf + warp * 32 * 17;
+    int done = 0;  // tiles so far
+    // the next tile's product may overwrite the output: also from the start
+    if (lane == 0) mbar_arrive(&sh->p_full[0]);
+    if (warp == CHUNK_WARP_OUT && lane == 0) a.split[blockIdx.x * 8] = 0;
+    for (bool more = first(); more; more = next()) {
+      const int n = c.j1 - c.j0, seg = c.seg;
+      const int live_rows = min(tt, c.q.n_q - c.rt * tt) * a.group;
+      const bool warp_live = quarter * 32 < live_rows, live = row < live_rows;
+      // keys from the segment's first on that the row sees
+      const int seen0 =
+          live ? c.q.kv_len - c.q.n_q + c.rt * tt + row / a.group + 1 - c.j0 * BN : 0;
+      const int item0 = ES == 4 ? 2 * (int)(c.unit + c.j0 - sh->begin) : 0;
       unsigned long long o2[HD / 2];  // the output, dims 2 i and 2 i + 1
-      float m = -INFINITY, l = 0.0f;
-      const int seen0 = see - c.j0 * BN;  // keys from the segment's first on that the row sees
+      float M = -INFINITY;            // what it is relative to
 #pragma unroll
       for (int d = 0; d < HD / 2; ++d) o2[d] = 0ull;
-      for (int j = w; j < n; j += 2, ++done) {
-        ok = __all_sync(0xffffffffu, chunk_wait(&sh->s_full[w], done & 1, sh, a, 49));
-        if (!ok) break;
-        tc_fence_after();
-        const int seen = min(max(seen0 - j * BN, 0), BN);
-        float corr = 1.0f, vs = 1.0f;
-        const bool whole = __all_sync(0xffffffffu, seen == BN || !live);
-        // the tile's K and V among the loaded items (a loader is at most NS + 4
-        // items ahead of the softmax groups)
-        const int item0 = ES == 4 ? 2 * (int)(c.unit + c.j0 - sh->begin) : 0;
-        const int item_k = item0 + (j == 0 ? 0 : 2 * j - 1);
-        const int item_v = item0 + (j == n - 1 ? 2 * n - 1 : 2 * j + 2);
-        if (warp_live) {
-          float ks = sc;
-          if constexpr (ES == 4) ks *= *(volatile float*)&sh->scale[item_k & 31];
-          // both passes over the scores load 16 columns ahead
-          float mx = -INFINITY;
-          uint32_t v0[16], v1[16];
-          tmem_ld16(t_s, v0);
-          tmem_wait_ld16(v0);
-          if (whole) {
-            float m2 = -INFINITY;
-#pragma unroll 1
-            for (int h = 0; h < BN; h += 32) {
-              tmem_ld16(t_s + h + 16, v1);
-#pragma unroll
-              for (int i = 0; i < 16; i += 4) {
-                mx = max3(mx, __uint_as_float(v0[i]), __uint_as_float(v0[i + 1]));
-                m2 = max3(m2, __uint_as_float(v0[i + 2]), __uint_as_float(v0[i + 3]));
-              }
-              tmem_wait_ld16(v1);
-              tmem_ld16(t_s + ((h + 32) & (BN - 1)), v0);  // at the end: the first again
-#pragma unroll
-              for (int i = 0; i < 16; i += 4) {
-                mx = max3(mx, __uint_as_float(v1[i]), __uint_as_float(v1[i + 1]));
-                m2 = max3(m2, __uint_as_float(v1[i + 2]), __uint_as_float(v1[i + 3]));
-              }
-              tmem_wait_ld16(v0);
-            }
-            mx = fmaxf(mx, m2);
-          } else {
-#pragma unroll 1
-            for (int h = 0; h < BN; h += 16) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (h + i < seen) mx = fmaxf(mx, __uint_as_float(v0[i]));
-              tmem_ld16(t_s + ((h + 16) & (BN - 1)), v0);
-              tmem_wait_ld16(v0);
-            }
-          }
-          const float mn = fmaxf(m, mx * ks);
-          const float mu = mn == -INFINITY ? 0.0f : mn;
-          corr = m == -INFINITY ? 0.0f : ex2(m - mu);
-          m = mn;
-          const float off = 13.0f - mu;
-          const unsigned long long ks2 = pk2(ks, ks), off2 = pk2(off, off);
-          const unsigned long long neg2 = pk2(-1.0f, -1.0f);
-          unsigned long long sum = 0ull, sum2 = 0ull;  // pairs of fp32
-          // weights of 16 keys from their scores v, stored over them
-          auto weigh = [&](const uint32_t* v, int h) {
-            uint32_t ph[8], pl[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float2 t = upk2(
-                  fma2(pk2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ks2, off2));
-              float x = ex2(t.x), y = ex2(t.y);
-              if (!whole) {
-                if (h + 2 * i >= seen) x = 0.0f;
-                if (h + 2 * i + 1 >= seen) y = 0.0f;
-              }
-              const unsigned long long p2 = pk2(x, y);
-              if (i & 1)
-                sum2 = add2(sum2, p2);
-              else
-                sum = add2(sum, p2);
-              ph[i] = pack_h2(x, y);
-              const float2 b = unpack_h2(ph[i]);
-              const float2 r = upk2(fma2(pk2(b.x, b.y), neg2, p2));
-              pl[i] = pack_h2(r.x, r.y);
-            }
-            tmem_st8(t_s + h, ph);
-            tmem_st8(t_s + h + 8, pl);
-          };
-#pragma unroll 1
-          for (int h = 0; h < BN; h += 32) {
-            tmem_ld16(t_s + h + 16, v1);
-            weigh(v0, h);
-            tmem_wait_ld16(v1);
-            if (h + 32 < BN) tmem_ld16(t_s + h + 32, v0);
-            weigh(v1, h + 16);
-            tmem_wait_ld16(v0);
-          }
-          const float2 total = upk2(add2(sum, sum2));
-          l = fmaf(l, corr, total.x + total.y);
-          tmem_wait_st();
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->p_full[w]);
-        ok = __all_sync(0xffffffffu, chunk_wait(&sh->o_full[w], done & 1, sh, a, 50));
+      for (int j = 0; j < n; ++j, ++done) {
+        ok = wait(&sh->o_full, done, 50);
         if (!ok) break;
         tc_fence_after();
         if (warp_live) {
-          if constexpr (ES == 4) vs = *(volatile float*)&sh->scale[item_v & 31];
-          bool odd = false;
-          if (!whole) {  // did an unseen NaN or infinity come in?
+          const float mt = sh->m_tile[done & 3][row];
+          float vs = 1.0f;  // (a loader is at most NS + 6 items ahead)
+          if constexpr (ES == 4)
+            vs = *(volatile float*)&sh->scale[(item0 + (j == n - 1 ? 2 * n - 1 : 2 * j + 2)) & 31];
+          const int seen = min(max(seen0 - j * BN, 0), BN);
+          if (!__all_sync(0xffffffffu, seen == BN || !live)) {
+            bool odd = false;  // did an unseen NaN or infinity come in?
 #pragma unroll 1
             for (int dc = 0; dc < HD; dc += 16) {
               uint32_t v[16];
               tmem_ld16(t_o + dc, v);
-              tmem_wait_ld();
+              tmem_wait_ld16(v);
 #pragma unroll
-              for (int i = 0; i < 16; ++i)
-                odd |= !(fabsf(__uint_as_float(v[i])) <= 3.4028235e38f);
+              for (int i = 0; i < 16; ++i) odd |= !(fabsf(__uint_as_float(v[i])) <= 3.4028235e38f);
             }
             odd = odd && live && seen < BN;
-          }
-          if (__any_sync(0xffffffffu, odd)) {
-            const int kb = (c.j0 + j) * BN;
-            const float* qrow = a.q + ((long long)c.q.q0 + c.rt * tt + row / a.group) * a.ldq +
-                                (size_t)(c.kvh * a.group + row % a.group) * HD;
-            int page = 0;
-            if (seen > 0)
-              page = c.q.pages[((size_t)a.layer * a.hkv + c.kvh) * c.q.pps + kb / KV_PAGE];
-            const bool in = page >= 0 && page < c.q.n_pages;
-            const KT* rows = reinterpret_cast<const KT*>(c.q.pool) +
-                             ((size_t)(in ? page : 0) * KV_PAGE + (kb & (KV_PAGE - 1))) * 2 * HD;
+            if (__any_sync(0xffffffffu, odd)) {
+              const int kb = (c.j0 + j) * BN;
+              const float* qrow = a.q + ((long long)c.q.q0 + c.rt * tt + row / a.group) * a.ldq +
+                                  (size_t)(c.kvh * a.group + row % a.group) * HD;
+              int page = 0;
+              if (seen > 0)
+                page = c.q.pages[((size_t)a.layer * a.hkv + c.kvh) * c.q.pps + kb / KV_PAGE];
+              const bool in = page >= 0 && page < c.q.n_pages;
+              const KT* rows = reinterpret_cast<const KT*>(c.q.pool) +
+                               ((size_t)(in ? page : 0) * KV_PAGE + (kb & (KV_PAGE - 1))) * 2 * HD;
 #pragma unroll 1
-            for (int dc = 0; dc < HD; dc += 16) {
-              uint32_t v[16];
-              tmem_ld16(t_o + dc, v);
-              tmem_wait_ld();
-              if (odd) {
-                chunk_row_slow<HD, KT>(rows, in ? seen : 0, qrow, a.scale, m, dc, tb + lane * 33);
+              for (int dc = 0; dc < HD; dc += 16) {
+                uint32_t v[16];
+                tmem_ld16(t_o + dc, v);
+                tmem_wait_ld16(v);
+                if (odd) {
+                  chunk_row_slow<HD, KT>(rows, in ? seen : 0, qrow, a.scale, mt, dc, tb + lane * 17);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(tb[lane * 33 + i] / vs);
+                  for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(tb[lane * 17 + i] / vs);
+                }
+                __syncwarp();
+                tmem_st16(t_o + dc, v);
               }
-              __syncwarp();
-              tmem_st8(t_o + dc, v);
-              tmem_st8(t_o + dc + 8, v + 8);
+              tmem_wait_st();
             }
-            tmem_wait_st();
           }
-          const unsigned long long corr2 = pk2(corr, corr), vs2 = pk2(vs, vs);
+          const float mn = fmaxf(M, mt);
+          const float co = M == -INFINITY ? 0.0f : ex2(M - mn);
+          const float ct = mt == -INFINITY ? 0.0f : ex2(mt - mn) * vs;
+          M = mn;
+          const unsigned long long co2 = pk2(co, co), ct2 = pk2(ct, ct);
 #pragma unroll
           for (int dc = 0; dc < HD; dc += 32) {
             uint32_t v[32];
             tmem_ld32(t_o + dc, v);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const unsigned long long t = pk2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-              if constexpr (ES == 4)
-                o2[dc / 2 + i] = fma2(t, vs2, mul2(o2[dc / 2 + i], corr2));
-              else
-                o2[dc / 2 + i] = fma2(o2[dc / 2 + i], corr2, t);
-            }
+            for (int i = 0; i < 16; ++i)
+              o2[dc / 2 + i] =
+                  fma2(pk2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ct2,
+                       mul2(o2[dc / 2 + i], co2));
           }
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->o_free[w]);
+        if (lane == 0) mbar_arrive(&sh->p_full[done + 1 & 1]);
       }
       if (!ok) break;
-
-      // the groups swap halves of their outputs through tensor memory: group 0
-      // finishes dims [0, HD / 2), group 1 the others
-      constexpr int HH = HD / 2;
-      // the other group has read its tile outputs of this segment (every
-      // product is complete then, and its warps are past the exchange of the
-      // segment before)
-      theirs += (n + w) / 2;
-      if (theirs > 0)
-        ok = __all_sync(0xffffffffu, chunk_wait(&sh->o_free[w ^ 1], (theirs - 1) & 1, sh, a, 52));
+      ok = wait(&sh->l_full, seg, 51);
       if (!ok) break;
-      if (warp_live) {
-        sh->ml[w][row][0] = m;
-        sh->ml[w][row][1] = l;
+      float L = 0.0f;
 #pragma unroll
-        for (int dc = 0; dc < HH; dc += 16) {
-          uint32_t u[16];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 x = upk2(w == 0 ? o2[(HH + dc) / 2 + i] : o2[dc / 2 + i]);
-            u[2 * i] = __float_as_uint(x.x);
-            u[2 * i + 1] = __float_as_uint(x.y);
-          }
-          tmem_st16(t_mine + dc, u);
-        }
-        tmem_wait_st();
+      for (int g = 0; g < 4; ++g) {
+        const float mg = sh->m_team[g & 1][row];
+        L = fmaf(sh->l_group[g][row], mg == -INFINITY ? 0.0f : ex2(mg - M), L);
       }
-      tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->xchg);
-      ok = __all_sync(0xffffffffu, chunk_wait(&sh->xchg, seg & 1, sh, a, 51));
-      if (!ok) break;
-      tc_fence_after();
+      if (lane == 0) mbar_arrive(&sh->e_done);
       const bool split = c.j0 > 0 || c.j1 < c.nk;
       const bool bad = *(volatile int*)&sh->bad[seg & 15] == seg + 1;
       // a piece that begins its row tile goes to the CTA's second place
       const size_t place = 2 * (size_t)blockIdx.x + (c.j0 == 0 ? 1 : 0);
       if (warp_live) {
         const long long row0 = (long long)c.q.q0 + c.rt * tt;
-        const float m2 = sh->ml[w ^ 1][row][0], l2 = sh->ml[w ^ 1][row][1];
-        const float M = fmaxf(m, m2);
-        const float f = m == -INFINITY ? 0.0f : ex2(m - M);
-        const float f2 = m2 == -INFINITY ? 0.0f : ex2(m2 - M);
-        const float L = fmaf(l, f, l2 * f2);
         const float inv = split ? 1.0f : L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
-        if (split && live && w == 0) {
+        if (split && live) {
           a.part_ml[(place * CHUNK_BM + row) * 2] = bad ? __int_as_float(0x7fc00000) : M;
           a.part_ml[(place * CHUNK_BM + row) * 2 + 1] = L;
         }
-        constexpr int OC = HH < 32 ? HH : 32;  // dims written at a time
+        // through shared memory, 16 dims at a time, four lanes a row
+        const int rl = lane >> 2, d4 = (lane & 3) * 4;
 #pragma unroll
-        for (int dc = 0; dc < HH; dc += OC) {
+        for (int dc = 0; dc < HD; dc += 16) {
+          __syncwarp();
 #pragma unroll
-          for (int e = 0; e < OC; e += 16) {
-            uint32_t v[16];
-            tmem_ld16(t_theirs + dc + e, v);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float2 x =
-                  upk2(w == 0 ? o2[(dc + e) / 2 + i] : o2[(HH + dc + e) / 2 + i]);
-              tb[lane * 33 + e + 2 * i] = fmaf(__uint_as_float(v[2 * i]), f2, x.x * f) * inv;
-              tb[lane * 33 + e + 2 * i + 1] = fmaf(__uint_as_float(v[2 * i + 1]), f2, x.y * f) * inv;
-            }
+          for (int i = 0; i < 8; ++i) {
+            const float2 x = upk2(o2[dc / 2 + i]);
+            tb[lane * 17 + 2 * i] = x.x * inv;
+            tb[lane * 17 + 2 * i + 1] = x.y * inv;
           }
           __syncwarp();
-          constexpr int LPR = OC / 4;  // lanes per row
-#pragma unroll
-          for (int i = 0; i < LPR; ++i) {
-            const int rl = i * (32 / LPR) + lane / LPR, r = (warp & 3) * 32 + rl;
-            const float* t = tb + rl * 33 + (lane % LPR) * 4;
+#pragma unroll 1
+          for (int i = 0; i < 32; i += 8) {
+            const int r = quarter * 32 + i + rl;
+            const float* t = tb + (i + rl) * 17 + d4;
             const float4 x = make_float4(t[0], t[1], t[2], t[3]);
-            const int d = w * HH + dc + (lane % LPR) * 4;
             if (r < live_rows) {
               if (split)
-                *reinterpret_cast<float4*>(a.part_o + (place * CHUNK_BM + r) * HD + d) = x;
+                *reinterpret_cast<float4*>(a.part_o + (place * CHUNK_BM + r) * HD + dc + d4) = x;
               else if (!bad)
                 *reinterpret_cast<float4*>(a.out + (row0 + r / a.group) * a.ldo +
-                                           (size_t)(c.kvh * a.group + r % a.group) * HD + d) = x;
+                                           (size_t)(c.kvh * a.group + r % a.group) * HD + dc + d4) =
+                    x;
             }
           }
-          __syncwarp();
         }
       }
-      tc_fence_before();
-      if (threadIdx.x == 0 && split && c.j1 == c.nk) {
+      if (warp == CHUNK_WARP_OUT && lane == 0 && split && c.j1 == c.nk) {
         // this CTA ends the row tile: what k_chunk_merge joins
         const long long sum = sh->pre[a.n_seqs];
         long long ctas = (sum + chunk_min_tiles(BN) - 1) / chunk_min_tiles(BN);
@@ -966,15 +786,213 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         d[3] = c.kvh;
         d[4] = c.rt;
       }
+    }
+  } else {
+    // ---- softmax ------------------------------------------------------------
+    regs_dec<CHUNK_R_SOFT>();
+    constexpr int KG = BN / 2;  // keys of a tile per thread
+    constexpr int DG = HD / 4;  // dims of q per group
+    const int g = warp >> 2, team = g & 1, half = g >> 1;
+    const uint32_t t_s = t_lane + CHUNK_T_S + team * BN + half * KG;
+    float* tb = tbuf + warp * 32 * 17;
+    int t0 = 0;            // tiles of the segments before
+    int qph = 0, mph = 0;  // phases of qx and mx
+    for (bool more = first(); more; more = next()) {
+      const int n = c.j1 - c.j0, seg = c.seg;
+      const int live_rows = min(tt, c.q.n_q - c.rt * tt) * a.group;
+      const bool warp_live = quarter * 32 < live_rows, live = row < live_rows;
+      // keys from the segment's first on that the row sees
+      const int seen0 =
+          live ? c.q.kv_len - c.q.n_q + c.rt * tt + row / a.group + 1 - c.j0 * BN : 0;
+      const int item0 = ES == 4 ? 2 * (int)(c.unit + c.j0 - sh->begin) : 0;
+      // the last product that reads the q before this is complete
+      if (t0 > 0) ok = wait(&sh->s_full[(t0 - 1) & 1], (t0 - 1) >> 1, 53);
+      if (!ok) break;
+      tc_fence_after();
+      float sc = 0.0f;
+      if (warp_live) {
+        // eight lanes read a row, four rows at a time, all in flight at once;
+        // group g takes the dims [g DG, g DG + DG); the terms go through shared
+        // memory to one row per lane
+        const int rl4 = lane >> 3, l8 = lane & 7;
+        constexpr int VL = DG / 8;  // floats of a row per lane
+        float x[8][VL];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = quarter * 32 + i * 4 + rl4;
+          const float* src = a.q + ((long long)c.q.q0 + c.rt * tt + r / a.group) * a.ldq +
+                             (size_t)(c.kvh * a.group + r % a.group) * HD + g * DG + l8 * VL;
+          if constexpr (VL == 4) {
+            const float4 y = r < live_rows ? *reinterpret_cast<const float4*>(src)
+                                           : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[i][0] = y.x, x[i][1] = y.y, x[i][2] = y.z, x[i][3] = y.w;
+          } else {
+#pragma unroll
+            for (int k = 0; k < VL; ++k) x[i][k] = r < live_rows ? src[k] : 0.0f;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float m = 0.0f;
+#pragma unroll
+          for (int k = 0; k < VL; ++k) m = fmaxf(m, fabsf(x[i][k]));
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          if (l8 == 0) sh->qmax[g][quarter * 32 + i * 4 + rl4] = m;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->qx[quarter]);
+        ok = wait(&sh->qx[quarter], qph++, 54);
+        if (!ok) break;
+        // a row's largest value lands in [2^10, 2^11)
+        auto up_of = [&](int r) {
+          return pow2i(10 - exp_of(fmaxf(fmaxf(sh->qmax[0][r], sh->qmax[1][r]),
+                                         fmaxf(sh->qmax[2][r], sh->qmax[3][r]))));
+        };
+        sc = a.scale / up_of(row);
+        uint32_t* tw = reinterpret_cast<uint32_t*>(tb);
+        constexpr int W = DG / 2;  // packed words of a row's term, at most 16
+#pragma unroll 1
+        for (int term = 0; term < 2; ++term) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float up = up_of(quarter * 32 + i * 4 + rl4);
+            uint32_t* t = tw + (i * 4 + rl4) * 17;
+            if constexpr (VL > 1) {
+#pragma unroll
+              for (int k = 0; k < VL; k += 2) {
+                const float y0 = x[i][k] * up, y1 = x[i][k + 1] * up;
+                uint32_t p = pack_h2(y0, y1);
+                if (term == 1) {
+                  const float2 b = unpack_h2(p);
+                  p = pack_h2(y0 - b.x, y1 - b.y);
+                }
+                t[l8 * (VL / 2) + k / 2] = p;
+              }
+            } else {
+              const float y = x[i][0] * up;
+              const __half h = __float2half_rn(y);
+              reinterpret_cast<__half*>(t)[l8] =
+                  term == 0 ? h : __float2half_rn(y - __half2float(h));
+            }
+          }
+          __syncwarp();
+          uint32_t u[W];
+#pragma unroll
+          for (int i = 0; i < W; ++i) u[i] = tw[lane * 17 + i];
+          tmem_stn<W>(t_lane + CHUNK_T_Q + term * (HD / 2) + g * W, u);
+        }
+        tmem_wait_st();
+      }
+      tc_fence_before();
       __syncwarp();
-      if (lane == 0) more = chunk_next<BN>(a, sh, c);
+      if (lane == 0) mbar_arrive(&sh->q_ready);
+
+      float m = -INFINITY, l = 0.0f;  // the team's maximum, this thread's sum
+      for (int j = (t0 ^ team) & 1; j < n; j += 2) {
+        const int tile = t0 + j;
+        ok = wait(&sh->s_full[team], tile >> 1, 49);
+        if (!ok) break;
+        tc_fence_after();
+        if (warp_live) {
+          // this thread's keys of the tile that the row sees
+          const int seen = min(max(seen0 - j * BN - half * KG, 0), KG);
+          const bool whole = __all_sync(0xffffffffu, seen == KG || !live);
+          float ks = sc;  // (a loader is at most NS + 6 items ahead)
+          if constexpr (ES == 4)
+            ks *= *(volatile float*)&sh->scale[(item0 + (j == 0 ? 0 : 2 * j - 1)) & 31];
+          float mx = -INFINITY;
+          if (whole) {
+            float m2 = -INFINITY;
+            uint32_t v[32];
+#pragma unroll
+            for (int h = 0; h < KG; h += 32) {
+              tmem_ld32(t_s + h, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                mx = max3(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                m2 = max3(m2, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+              }
+            }
+            mx = fmaxf(mx, m2);
+          } else {
+#pragma unroll 1
+            for (int h = 0; h < KG; h += 16) {
+              uint32_t v[16];
+              tmem_ld16(t_s + h, v);
+              tmem_wait_ld16(v);
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (h + i < seen) mx = fmaxf(mx, __uint_as_float(v[i]));
+            }
+          }
+          // the row's other half of the keys
+          const int gb = tile >> 1 & 1;
+          sh->gmax[team][gb][half][row] = mx;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->mx[team][quarter]);
+          ok = wait(&sh->mx[team][quarter], mph++, 55);
+          if (!ok) break;
+          mx = fmaxf(mx, sh->gmax[team][gb][half ^ 1][row]);
+          const float mn = fmaxf(m, mx * ks);
+          const float mu = mn == -INFINITY ? 0.0f : mn;
+          l *= m == -INFINITY ? 0.0f : ex2(m - mu);
+          m = mn;
+          if (half == 0) sh->m_tile[tile & 3][row] = m;
+          const float off = 13.0f - mu;
+          const unsigned long long ks2 = pk2(ks, ks), off2 = pk2(off, off);
+          const unsigned long long neg2 = pk2(-1.0f, -1.0f);
+          unsigned long long sum = 0ull;  // a pair of fp32
+#pragma unroll 1
+          for (int h = 0; h < KG; h += 16) {
+            uint32_t v[16], ph[8], pl[8];
+            tmem_ld16(t_s + h, v);
+            tmem_wait_ld16(v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float2 t = upk2(
+                  fma2(pk2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ks2, off2));
+              float x = ex2(t.x), y = ex2(t.y);
+              if (!whole) {
+                if (h + 2 * i >= seen) x = 0.0f;
+                if (h + 2 * i + 1 >= seen) y = 0.0f;
+              }
+              const unsigned long long p2 = pk2(x, y);
+              sum = add2(sum, p2);
+              ph[i] = pack_h2(x, y);
+              const float2 b = unpack_h2(ph[i]);
+              const float2 r = upk2(fma2(pk2(b.x, b.y), neg2, p2));
+              pl[i] = pack_h2(r.x, r.y);
+            }
+            tmem_st8(t_s + h, ph);
+            tmem_st8(t_s + h + 8, pl);
+          }
+          const float2 total = upk2(sum);
+          l += total.x + total.y;
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->p_full[team]);
+      }
+      if (!ok) break;
+      t0 += n;
+      // the statistics, once those of the segment before have been read
+      if (seg > 0) ok = wait(&sh->e_done, seg - 1, 52);
+      if (!ok) break;
+      sh->l_group[g][row] = l;
+      if (half == 0) sh->m_team[team][row] = m;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->l_full);
     }
   }
   cp_async_wait<0>();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 15) {
+  if (warp == CHUNK_WARP_MMA) {
     __syncwarp();
     tmem_dealloc(tmem, CHUNK_T_COLS);
   }
