@@ -50,6 +50,7 @@ struct ChunkArgs {
   float* out;
   long long ldo;
   int layer, hkv, group;
+  int ginv;          // row / group = row * ginv >> 16 for the rows of a tile
   float scale;       // of the scores, times log2 e
   float* part_o;     // [2 * grid][128][HD] outputs of split row tiles
   float* part_ml;    // [2 * grid][128][2] their maxima and sums
@@ -72,8 +73,11 @@ struct ChunkCursor {
 
 struct ChunkSmem {
   uint8_t map[CHUNK_LOAD][128];  // (at the start: 128-byte aligned)
-  uint64_t full[CHUNK_LOAD], empty[CHUNK_LOAD], raw[CHUNK_LOAD];  // K / V slots
-  uint64_t s_full[2], p_full[2], o_full;
+  uint64_t empty[CHUNK_LOAD], raw[CHUNK_LOAD];  // K / V slots
+  // of tile t, at t & 7: its K tile is there and the weights that lie over its S
+  // are spent; its V tile and weights are there and the output before is read
+  uint64_t s_go[8], o_go[8];
+  uint64_t s_full[2], o_full;
   uint64_t q_ready, l_full, e_done, drain;
   uint64_t qx[4], mx[2][4];      // per quarter of the rows: its groups met
   uint32_t tmem_base;
@@ -354,14 +358,16 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&sh->full[i], 1);
       mbar_init(&sh->empty[i], 1);
       mbar_init(&sh->raw[i], 1);
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(&sh->s_full[w], 1);
-      mbar_init(&sh->p_full[w], CHUNK_SOFT / 2 + CHUNK_OUT);
       for (int i = 0; i < 4; ++i) mbar_init(&sh->mx[w][i], 2);
+    }
+    for (int i = 0; i < 8; ++i) {
+      mbar_init(&sh->s_go[i], 2);
+      mbar_init(&sh->o_go[i], 1 + CHUNK_SOFT / 2 + CHUNK_OUT);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&sh->qx[i], 4);
     mbar_init(&sh->o_full, 1);
@@ -372,6 +378,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     sh->abort_flag = 0;
     for (int i = 0; i < 16; ++i) sh->bad[i] = 0;
     fence_mbar_init();
+    mbar_arrive(&sh->s_go[0]);  // nothing lies over the first two S
+    mbar_arrive(&sh->s_go[1]);
   }
   if (warp == 0) {
     __syncwarp();
@@ -451,7 +459,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           map_pool = c.q.pool;
           tmap_rebase(map, sh->map[lw], &a.map, map_pool, lane);
         }
-        uint64_t* landed = ES == 2 ? &sh->full[lw] : &sh->raw[lw];
+        const int tile = (it0 >> 1) + j - c.j0;
+        uint64_t* go = is_v ? &sh->o_go[tile & 7] : &sh->s_go[tile & 7];
+        uint64_t* landed = ES == 2 ? go : &sh->raw[lw];
         if (cnt == BN) {
           if (lane == 0) {
             mbar_arrive_expect_tx(landed, SLOT);
@@ -533,7 +543,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             }
           fence_proxy_async_shared();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sh->full[lw]);
+          if (lane == 0) mbar_arrive(go);
         }
       }
       it0 += 2 * n;
@@ -551,25 +561,18 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     constexpr uint64_t DESC_K = gemm::smem_desc(0, 16, 8 * RB) | SWZ;
     constexpr uint64_t DESC_V = gemm::smem_desc(0, NEXT, 8 * RB) | SWZ;
     const uint32_t ring0 = smem_u32(ring) >> 4;
-    // The whole warp walks the loop, one lane issues.  The tensor core takes
-    // new products only while it has few left, so what a batch needs is waited
-    // for as early as its order allows.
+    // The whole warp walks the loop, one lane issues.  The tensor core takes new
+    // products only while it has about four left (280 cycles), so a batch has
+    // one barrier for all that it needs: a wait takes 100 to 200.
     int it = 0;          // slots used
     int ns = 0, no = 0;  // tiles so far, issued to S and to O
     for (bool more = first(); more && ok; more = next()) {
       const int n = __shfl_sync(0xffffffffu, c.j1 - c.j0, 0);
       ok = wait(&sh->q_ready, c.seg, 42);
-      // at a segment's start every product so far is complete
-      if (ok && ns > 0) ok = wait(&sh->o_full, ns - 1, 44);
       for (int j = 0; j <= n && ok; ++j) {
-        const int slot = it % NS, slot2 = (it + 1) % NS;
-        ok = wait(&sh->full[slot], it / NS, 43);
-        if (ok && j >= 1 && j < n) ok = wait(&sh->full[slot2], (it + 1) / NS, 45);
         if (j < n) {
-          const int w = ns & 1;
-          // the weights of the tile before the last lie over S until their
-          // product is complete
-          if (ok && j > 1) ok = wait(&sh->o_full, ns - 2, 44);
+          const int w = ns & 1, slot = it % NS;
+          ok = wait(&sh->s_go[ns & 7], ns >> 3, 43);
           if (!ok) break;
           tc_fence_after();
           const uint32_t b0 = ring0 + (uint32_t)(slot * (SLOT >> 4)) + (uint32_t)DESC_K;
@@ -597,12 +600,11 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           ++it;
         }
         if (j >= 1) {
-          const int w = no & 1, vs = j < n ? slot2 : slot;
-          // the weights are there and the output of the tile before has been read
-          ok = wait(&sh->p_full[w], no >> 1, 46);
+          const int w = no & 1, slot = it % NS;
+          ok = wait(&sh->o_go[no & 7], no >> 3, 46);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t b0 = ring0 + (uint32_t)(vs * (SLOT >> 4)) + (uint32_t)DESC_V;
+          const uint32_t b0 = ring0 + (uint32_t)(slot * (SLOT >> 4)) + (uint32_t)DESC_V;
           const uint32_t pw = tmem + CHUNK_T_S + w * BN;
           const uint32_t d = tmem + CHUNK_T_O;
           if (elect_one()) {
@@ -619,8 +621,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                   mma_f16_ts<true>(d, pa, bb + k * RB, (uint32_t)(DESC_V >> 32), IDESC_O);  // 16 keys
               }
             }
+            mma_commit(&sh->s_go[(no + 2) & 7]);
             mma_commit(&sh->o_full);
-            mma_commit(&sh->empty[vs]);
+            mma_commit(&sh->empty[slot]);
           }
           __syncwarp();
           ++no;
@@ -642,7 +645,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     float* tb = tbuf + warp * 32 * 17;
     int done = 0;  // tiles so far
     // the next tile's product may overwrite the output: also from the start
-    if (lane == 0) mbar_arrive(&sh->p_full[0]);
+    if (lane == 0) mbar_arrive(&sh->o_go[0]);
     if (warp == CHUNK_WARP_OUT && lane == 0) a.split[blockIdx.x * 8] = 0;
     for (bool more = first(); more; more = next()) {
       const int n = c.j1 - c.j0, seg = c.seg;
@@ -650,7 +653,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       const bool warp_live = quarter * 32 < live_rows, live = row < live_rows;
       // keys from the segment's first on that the row sees
       const int seen0 =
-          live ? c.q.kv_len - c.q.n_q + c.rt * tt + row / a.group + 1 - c.j0 * BN : 0;
+          live ? c.q.kv_len - c.q.n_q + c.rt * tt + (row * a.ginv >> 16) + 1 - c.j0 * BN : 0;
       const int item0 = ES == 4 ? 2 * (int)(c.unit + c.j0 - sh->begin) : 0;
       unsigned long long o2[HD / 2];  // the output, dims 2 i and 2 i + 1
       float M = -INFINITY;            // what it is relative to
@@ -708,21 +711,41 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           const float ct = mt == -INFINITY ? 0.0f : ex2(mt - mn) * vs;
           M = mn;
           const unsigned long long co2 = pk2(co, co), ct2 = pk2(ct, ct);
+          const bool same = __all_sync(0xffffffffu, co == 1.0f);
+          // 16 columns ahead; the next product may overwrite them once the last
+          // are loaded
+          uint32_t v0[16], v1[16];
+          auto add = [&](const uint32_t* v, int dc) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const unsigned long long t =
+                  pk2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+              unsigned long long& o = o2[dc / 2 + i];
+              if (!same) o = mul2(o, co2);
+              o = fma2(t, ct2, o);
+            }
+          };
+          tmem_ld16(t_o, v0);
+          tmem_wait_ld16(v0);
 #pragma unroll
           for (int dc = 0; dc < HD; dc += 32) {
-            uint32_t v[32];
-            tmem_ld32(t_o + dc, v);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              o2[dc / 2 + i] =
-                  fma2(pk2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ct2,
-                       mul2(o2[dc / 2 + i], co2));
+            tmem_ld16(t_o + dc + 16, v1);
+            add(v0, dc);
+            tmem_wait_ld16(v1);
+            if (dc + 32 < HD) tmem_ld16(t_o + dc + 32, v0);
+            if (dc + 32 >= HD) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sh->o_go[(done + 1) & 7]);
+            }
+            add(v1, dc + 16);
+            if (dc + 32 < HD) tmem_wait_ld16(v0);
           }
+        } else {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->o_go[(done + 1) & 7]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->p_full[done + 1 & 1]);
       }
       if (!ok) break;
       ok = wait(&sh->l_full, seg, 51);
@@ -741,6 +764,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       const size_t place = 2 * (size_t)blockIdx.x + (c.j0 == 0 ? 1 : 0);
       if (warp_live) {
         const long long row0 = (long long)c.q.q0 + c.rt * tt;
+        const int head0 = c.kvh * a.group;
         const float inv = split ? 1.0f : L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
         if (split && live) {
           a.part_ml[(place * CHUNK_BM + row) * 2] = bad ? __int_as_float(0x7fc00000) : M;
@@ -760,16 +784,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           __syncwarp();
 #pragma unroll 1
           for (int i = 0; i < 32; i += 8) {
-            const int r = quarter * 32 + i + rl;
+            const int r = quarter * 32 + i + rl, tok = r * a.ginv >> 16;
             const float* t = tb + (i + rl) * 17 + d4;
             const float4 x = make_float4(t[0], t[1], t[2], t[3]);
             if (r < live_rows) {
               if (split)
                 *reinterpret_cast<float4*>(a.part_o + (place * CHUNK_BM + r) * HD + dc + d4) = x;
               else if (!bad)
-                *reinterpret_cast<float4*>(a.out + (row0 + r / a.group) * a.ldo +
-                                           (size_t)(c.kvh * a.group + r % a.group) * HD + dc + d4) =
-                    x;
+                *reinterpret_cast<float4*>(a.out + (row0 + tok) * a.ldo +
+                                           (size_t)(head0 + r - tok * a.group) * HD + dc + d4) = x;
             }
           }
         }
@@ -803,7 +826,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       const bool warp_live = quarter * 32 < live_rows, live = row < live_rows;
       // keys from the segment's first on that the row sees
       const int seen0 =
-          live ? c.q.kv_len - c.q.n_q + c.rt * tt + row / a.group + 1 - c.j0 * BN : 0;
+          live ? c.q.kv_len - c.q.n_q + c.rt * tt + (row * a.ginv >> 16) + 1 - c.j0 * BN : 0;
       const int item0 = ES == 4 ? 2 * (int)(c.unit + c.j0 - sh->begin) : 0;
       // the last product that reads the q before this is complete
       if (t0 > 0) ok = wait(&sh->s_full[(t0 - 1) & 1], (t0 - 1) >> 1, 53);
@@ -811,6 +834,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       tc_fence_after();
       float sc = 0.0f;
       if (warp_live) {
+        const long long row0 = (long long)c.q.q0 + c.rt * tt;
+        const int head0 = c.kvh * a.group;
         // eight lanes read a row, four rows at a time, all in flight at once;
         // group g takes the dims [g DG, g DG + DG); the terms go through shared
         // memory to one row per lane
@@ -820,8 +845,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int r = quarter * 32 + i * 4 + rl4;
-          const float* src = a.q + ((long long)c.q.q0 + c.rt * tt + r / a.group) * a.ldq +
-                             (size_t)(c.kvh * a.group + r % a.group) * HD + g * DG + l8 * VL;
+          const int tok = r * a.ginv >> 16;
+          const float* src = a.q + (row0 + tok) * a.ldq +
+                             (size_t)(head0 + r - tok * a.group) * HD + g * DG + l8 * VL;
           if constexpr (VL == 4) {
             const float4 y = r < live_rows ? *reinterpret_cast<const float4*>(src)
                                            : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -850,6 +876,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                                          fmaxf(sh->qmax[2][r], sh->qmax[3][r]))));
         };
         sc = a.scale / up_of(row);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float up = up_of(quarter * 32 + i * 4 + rl4);
+#pragma unroll
+          for (int k = 0; k < VL; ++k) x[i][k] *= up;
+        }
         uint32_t* tw = reinterpret_cast<uint32_t*>(tb);
         constexpr int W = DG / 2;  // packed words of a row's term, at most 16
 #pragma unroll 1
@@ -857,12 +889,11 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float up = up_of(quarter * 32 + i * 4 + rl4);
             uint32_t* t = tw + (i * 4 + rl4) * 17;
             if constexpr (VL > 1) {
 #pragma unroll
               for (int k = 0; k < VL; k += 2) {
-                const float y0 = x[i][k] * up, y1 = x[i][k + 1] * up;
+                const float y0 = x[i][k], y1 = x[i][k + 1];
                 uint32_t p = pack_h2(y0, y1);
                 if (term == 1) {
                   const float2 b = unpack_h2(p);
@@ -871,7 +902,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                 t[l8 * (VL / 2) + k / 2] = p;
               }
             } else {
-              const float y = x[i][0] * up;
+              const float y = x[i][0];
               const __half h = __float2half_rn(y);
               reinterpret_cast<__half*>(t)[l8] =
                   term == 0 ? h : __float2half_rn(y - __half2float(h));
@@ -975,7 +1006,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->p_full[team]);
+        if (lane == 0) mbar_arrive(&sh->o_go[tile & 7]);
       }
       if (!ok) break;
       t0 += n;

@@ -190,6 +190,7 @@ extern "C" int l3g_chunk_attn_run(l3g_chunk_attn* h, const l3g_chunk_seq* seqs, 
   a.layer = layer;
   a.hkv = h->hkv;
   a.group = h->heads / h->hkv;
+  a.ginv = 65535 / a.group + 1;
   a.scale = (float)((scale > 0.0f ? (double)scale : 1.0 / sqrt((double)h->hd)) * M_LOG2E);
   a.res = h->d_res;
   a.part_o = h->part_o;

@@ -136,6 +136,7 @@ int emu_chunk_attention(const void* seqs, int n_seqs, int total_q, const float* 
     a.layer = layer;
     a.hkv = hkv;
     a.group = heads / hkv;
+    a.ginv = 65535 / a.group + 1;
     a.scale = (float)(scale * M_LOG2E);
     a.part_o = static_cast<float*>(dm((size_t)2 * grid * 128 * hd * 4));
     a.part_ml = static_cast<float*>(dm((size_t)2 * grid * 128 * 2 * 4));
