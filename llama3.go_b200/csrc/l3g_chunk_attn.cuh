@@ -79,7 +79,8 @@ struct ChunkSmem {
   uint64_t s_go[8], o_go[8];
   uint64_t s_full[2], o_full;
   uint64_t q_ready, l_full, e_done, drain;
-  uint64_t qx[4], mx[2][4];      // per quarter of the rows: its groups met
+  // per quarter of the rows: its four groups met, its team's two met
+  uint64_t qx[4], mx[2][4];
   uint32_t tmem_base;
   int abort_flag;
   int n_tiles_lo, pad;
@@ -95,7 +96,7 @@ struct ChunkSmem {
   float m_team[2][CHUNK_BM], l_group[4][CHUNK_BM];  // a segment's statistics
   long long pre[L3G_CHUNK_SEQS_MAX + 1];  // tiles before each sequence
 };
-constexpr int CHUNK_HEAD = 20 * 1024;
+constexpr int CHUNK_HEAD = 24 * 1024;
 static_assert(sizeof(ChunkSmem) <= CHUNK_HEAD, "chunk attention smem head");
 constexpr int CHUNK_TBUF = 32 * 17 * 4;  // a softmax or output warp's transposition buffer
 __host__ __device__ constexpr int chunk_slot_bytes(int hd, int es) {
@@ -361,6 +362,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       mbar_init(&sh->empty[i], 1);
       mbar_init(&sh->raw[i], 1);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&sh->qx[i], 4);
     for (int w = 0; w < 2; ++w) {
       mbar_init(&sh->s_full[w], 1);
       for (int i = 0; i < 4; ++i) mbar_init(&sh->mx[w][i], 2);
@@ -369,7 +371,6 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       mbar_init(&sh->s_go[i], 2);
       mbar_init(&sh->o_go[i], 1 + CHUNK_SOFT / 2 + CHUNK_OUT);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&sh->qx[i], 4);
     mbar_init(&sh->o_full, 1);
     mbar_init(&sh->q_ready, CHUNK_SOFT);
     mbar_init(&sh->l_full, CHUNK_SOFT);
@@ -427,7 +428,17 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     int it = lw;                  // this warp's next item
     int it0 = 0;                  // the segment's first
     ok = lw < NS;
-    for (bool more = first(); more && ok; more = next()) {
+    for (bool more = ok && first(); more && ok; more = next()) {
+      {  // the segment's q rows into L2, ahead of the softmax warps' loads
+        const int live_rows = min(tt, c.q.n_q - c.rt * tt) * a.group;
+        const float* q0 = a.q + ((long long)c.q.q0 + (long long)c.rt * tt) * a.ldq +
+                          (size_t)c.kvh * a.group * HD;
+        constexpr int LINES = HD / 32;  // of 128 bytes per row
+        for (int e = lw * 32 + lane; e < live_rows * LINES; e += NS * 32) {
+          const int r = e / LINES, tok = r * a.ginv >> 16;
+          prefetch_l2(q0 + tok * a.ldq + (r - tok * a.group) * HD + e % LINES * 32);
+        }
+      }
       const int n = c.j1 - c.j0;
       const int* pages = c.q.pages + ((size_t)a.layer * a.hkv + c.kvh) * c.q.pps;
       for (; it < it0 + 2 * n; it += NS) {
@@ -674,8 +685,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll 1
             for (int dc = 0; dc < HD; dc += 16) {
               uint32_t v[16];
-              tmem_ld16(t_o + dc, v);
-              tmem_wait_ld16(v);
+              tmem_get16(t_o + dc, v);
 #pragma unroll
               for (int i = 0; i < 16; ++i) odd |= !(fabsf(__uint_as_float(v[i])) <= 3.4028235e38f);
             }
@@ -693,8 +703,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll 1
               for (int dc = 0; dc < HD; dc += 16) {
                 uint32_t v[16];
-                tmem_ld16(t_o + dc, v);
-                tmem_wait_ld16(v);
+                tmem_get16(t_o + dc, v);
                 if (odd) {
                   chunk_row_slow<HD, KT>(rows, in ? seen : 0, qrow, a.scale, mt, dc, tb + lane * 17);
 #pragma unroll
@@ -712,34 +721,21 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           M = mn;
           const unsigned long long co2 = pk2(co, co), ct2 = pk2(ct, ct);
           const bool same = __all_sync(0xffffffffu, co == 1.0f);
-          // 16 columns ahead; the next product may overwrite them once the last
-          // are loaded
-          uint32_t v0[16], v1[16];
-          auto add = [&](const uint32_t* v, int dc) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const unsigned long long t =
-                  pk2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-              unsigned long long& o = o2[dc / 2 + i];
-              if (!same) o = mul2(o, co2);
-              o = fma2(t, ct2, o);
-            }
-          };
-          tmem_ld16(t_o, v0);
-          tmem_wait_ld16(v0);
 #pragma unroll
           for (int dc = 0; dc < HD; dc += 32) {
-            tmem_ld16(t_o + dc + 16, v1);
-            add(v0, dc);
-            tmem_wait_ld16(v1);
-            if (dc + 32 < HD) tmem_ld16(t_o + dc + 32, v0);
-            if (dc + 32 >= HD) {
+            uint32_t v[32];
+            tmem_get32(t_o + dc, v);
+            if (dc + 32 >= HD) {  // the next product may overwrite it
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(&sh->o_go[(done + 1) & 7]);
             }
-            add(v1, dc + 16);
-            if (dc + 32 < HD) tmem_wait_ld16(v0);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              unsigned long long& o = o2[dc / 2 + i];
+              if (!same) o = mul2(o, co2);
+              o = fma2(pk2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ct2, o);
+            }
           }
         } else {
           tc_fence_before();
@@ -939,8 +935,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             uint32_t v[32];
 #pragma unroll
             for (int h = 0; h < KG; h += 32) {
-              tmem_ld32(t_s + h, v);
-              tmem_wait_ld();
+              tmem_get32(t_s + h, v);
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
                 mx = max3(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
@@ -952,8 +947,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll 1
             for (int h = 0; h < KG; h += 16) {
               uint32_t v[16];
-              tmem_ld16(t_s + h, v);
-              tmem_wait_ld16(v);
+              tmem_get16(t_s + h, v);
 #pragma unroll
               for (int i = 0; i < 16; ++i)
                 if (h + i < seen) mx = fmaxf(mx, __uint_as_float(v[i]));
@@ -976,17 +970,16 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           const unsigned long long ks2 = pk2(ks, ks), off2 = pk2(off, off);
           const unsigned long long neg2 = pk2(-1.0f, -1.0f);
           unsigned long long sum = 0ull;  // a pair of fp32
-#pragma unroll 1
-          for (int h = 0; h < KG; h += 16) {
+          // weights of 16 keys from h on, over their scores; ALL: the row sees them
+          auto weigh = [&](int h, auto all) {
             uint32_t v[16], ph[8], pl[8];
-            tmem_ld16(t_s + h, v);
-            tmem_wait_ld16(v);
+            tmem_get16(t_s + h, v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const float2 t = upk2(
                   fma2(pk2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ks2, off2));
               float x = ex2(t.x), y = ex2(t.y);
-              if (!whole) {
+              if constexpr (!decltype(all)::value) {
                 if (h + 2 * i >= seen) x = 0.0f;
                 if (h + 2 * i + 1 >= seen) y = 0.0f;
               }
@@ -999,6 +992,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             }
             tmem_st8(t_s + h, ph);
             tmem_st8(t_s + h + 8, pl);
+          };
+          if (whole) {
+#pragma unroll 1
+            for (int h = 0; h < KG; h += 16) weigh(h, std::true_type());
+          } else {
+#pragma unroll 1
+            for (int h = 0; h < KG; h += 16) weigh(h, std::false_type());
           }
           const float2 total = upk2(sum);
           l += total.x + total.y;

@@ -2,6 +2,8 @@
 // probabilities, page copies.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "l3g_rt.h"
 
 namespace l3g {

@@ -4,6 +4,7 @@
 #include "simt.h"
 
 #include <cuda.h>
+#include <type_traits>
 
 #define execute_mma execute_mma_i8
 #include "simt_tcgen05.h"

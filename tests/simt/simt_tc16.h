@@ -20,6 +20,9 @@ inline void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t
   ::simt::queue_tensor_op(op);
 }
 inline bool mbar_try_wait(uint64_t* b, uint32_t parity, uint32_t) { return mbar_test(b, parity); }
+inline void prefetch_l2(const void* p) {
+  if (!::simt::in_global(p, 4)) ::simt::fail("prefetch outside every buffer");
+}
 inline bool elect_one() { return ::simt::cur()->lane == 0; }
 inline uint32_t* tmem_cell(uint32_t taddr, int cols) {
   ::simt::Thread* t = ::simt::cur();
@@ -32,9 +35,8 @@ inline uint32_t* tmem_cell(uint32_t taddr, int cols) {
     if (!(t->blk->tmem_used >> u & 1u)) ::simt::fail("tcgen05.ld/st of unallocated tensor memory");
   return &t->blk->tmem[(size_t)(lane0 + t->lane) * 512 + col];
 }
-inline void tmem_ld32(uint32_t taddr, uint32_t* v) { memcpy(v, tmem_cell(taddr, 32), 128); }
-inline void tmem_ld16(uint32_t taddr, uint32_t* v) { memcpy(v, tmem_cell(taddr, 16), 64); }
-inline void tmem_wait_ld16(uint32_t*) {}
+inline void tmem_get32(uint32_t taddr, uint32_t* v) { memcpy(v, tmem_cell(taddr, 32), 128); }
+inline void tmem_get16(uint32_t taddr, uint32_t* v) { memcpy(v, tmem_cell(taddr, 16), 64); }
 inline void tmem_st16(uint32_t taddr, const uint32_t* v) { memcpy(tmem_cell(taddr, 16), v, 64); }
 inline void tmem_st8(uint32_t taddr, const uint32_t* v) { memcpy(tmem_cell(taddr, 8), v, 32); }
 inline void tmem_st4(uint32_t taddr, const uint32_t* v) { memcpy(tmem_cell(taddr, 4), v, 16); }
