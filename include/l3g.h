@@ -530,8 +530,8 @@ int l3g_chunk_attn_status(l3g_chunk_attn *h, int32_t *err, int32_t *where);
  * (the order of ForwardTopKIntoWorkspace's items, topk.go).  -inf logits are
  * tokens of probability zero; a row of nothing else has entropy 0 and log
  * probabilities of -inf.  A row with a NaN or +inf has NaN for logprob, entropy
- * and top_logprobs, and in its order NaNs follow their sign bits beyond the
- * infinities.  A target outside [0, vocab) is none: logprob NaN, rank -1.
+ * and top_logprobs; among its alternatives NaNs follow their sign bits beyond
+ * the infinities, and its rank leaves NaNs out.  A target outside [0, vocab) is none: logprob NaN, rank -1.
  * logprob and rank (with targets), entropy, top_ids and top_logprobs may be
  * NULL; top_k in [0, 64], at most vocab.  ld >= vocab. */
 typedef struct l3g_logprobs l3g_logprobs;

@@ -1,17 +1,31 @@
 // Log probabilities of given tokens, entropy, rank and top alternatives of
 // logits rows (included by l3g_ops.cu inside namespace l3g).
+//
+// With m = max x, d_i = x_i - m, S = sum e^d_i, S1 = sum e^d_i d_i:
+//   log p_t = d_t - log S,   entropy = log S - S1 / S,
+// so one pass over the row is enough and nothing cancels (d_i <= 0).  A row is
+// cut into slices that a CTA holds in registers; slices with maxima m_a are
+// joined by S = sum_a S_a e^(m_a - m), S1 = sum_a (S1_a + S_a (m_a - m)) e^(m_a - m).
+// The pass is bound by memory: 4 bytes and about 16 instructions a value.
 #pragma once
+
+constexpr int LP_THREADS = 512;
+// Threads with a key at or above the threshold that the search stops at: k and
+// up to LP_SLACK more.
+constexpr int LP_SLACK = 16;
 
 struct LogprobArgs {
   const float* x;
   long long ld;
-  int n, vocab, k;
+  int n, vocab, k, slices;
   const int* targets;
   float* logprob;
   float* entropy;
   int* rank;
   int* top_ids;
   float* top_lp;
+  float4* part;     // [n][slices] {m, S, S1, tokens before the target (bits)}
+  uint64_t* part_k; // [n][slices][k] the slices' top keys, sorted
 };
 
 // The order of the alternatives: larger logit first, lower id on ties (-0
@@ -20,38 +34,112 @@ __device__ __forceinline__ uint64_t logit_key(float v, int idx) {
   return topk_key(v == 0.0f ? 0.0f : v, idx);
 }
 
-// One CTA of 256 threads per row: maximum, sums, rank, then one pass per
-// alternative.
-__global__ void k_logprobs_simple(const LogprobArgs a) {
-  __shared__ float red[8], red2[8];
-  __shared__ int redi[8];
-  __shared__ uint64_t redk[8];
-  const int r = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+// What a row's sums give.
+struct LogprobRow {
+  float m, s, s1;
+  int before;
+};
+__device__ __forceinline__ void logprob_write(const LogprobArgs& a, int r, const LogprobRow& w,
+                                              float xt, bool has_t, int tid) {
+  const bool none = w.m == -INFINITY && w.s == 0.0f;  // every token masked
+  if (tid != 0) return;
+  const float ls = logf(w.s);
+  if (a.logprob)
+    a.logprob[r] = !has_t ? __int_as_float(0x7fc00000) : none ? -INFINITY : xt - w.m - ls;
+  if (a.rank) a.rank[r] = has_t ? w.before : -1;
+  if (a.entropy) a.entropy[r] = none ? 0.0f : ls - w.s1 / w.s;
+}
+__device__ __forceinline__ void logprob_top(const LogprobArgs& a, int r, const LogprobRow& w,
+                                            uint64_t key, int place) {
+  const bool none = w.m == -INFINITY && w.s == 0.0f;
+  if (a.top_ids) a.top_ids[(size_t)r * a.k + place] = key_index(key);
+  if (a.top_lp)
+    a.top_lp[(size_t)r * a.k + place] = none ? -INFINITY : key_value(key) - w.m - logf(w.s);
+}
+
+// One slice of LP_THREADS * E values.  grid (slices, rows).  VEC: rows start on
+// 16-byte boundaries.
+//
+// The top k of the slice: the k-th largest of the threads' own largest values
+// is at or below the slice's k-th value, so every one of the top k belongs to a
+// thread whose largest is at or above it.  That threshold is bisected, on the
+// values' bits, until k to k + LP_SLACK threads are at or above it; their at
+// most (k + LP_SLACK) * E values at or above it are gathered as keys (value and
+// id) and each finds its place by counting the larger ones.  The work hardly
+// depends on the values: a descending row costs what a random one does.  Where
+// too many threads tie, or the slice holds a NaN or +inf, whole keys, which all
+// differ, are bisected instead.
+template <int E, bool VEC>
+__global__ void __launch_bounds__(LP_THREADS, E == 32 ? 2 : 3)
+    k_logprobs_part(const LogprobArgs a) {
+  constexpr int NWARP = LP_THREADS / 32;
+  constexpr int CAP = (MAX_TOPK + LP_SLACK) * E;
+  __shared__ float red[NWARP], red2[NWARP], redm[NWARP];
+  __shared__ int redi[NWARP], count;
+  __shared__ uint64_t lohi[2], cand[CAP];
+  const int r = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int base = blockIdx.x * LP_THREADS * E;
   const float* x = a.x + (long long)r * a.ld;
-  float m = -INFINITY;
-  for (int i = tid; i < a.vocab; i += 256) m = fmaxf(m, x[i]);
-  m = warp_max(m);
-  if (lane == 0) red[warp] = m;
-  __syncthreads();
-  for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
-  __syncthreads();
+  pdl_launch_dependents();
   const int t = a.targets ? a.targets[r] : -1;
   const bool has_t = t >= 0 && t < a.vocab;
   const float xt = has_t ? x[t] : 0.0f;
-  const uint64_t kt = has_t ? logit_key(xt, t) : ~0ull;
-  float s = 0.0f, s1 = 0.0f;
-  int before = 0;
-  for (int i = tid; i < a.vocab; i += 256) {
-    const float v = x[i], d = v - m;
-    if (v != -INFINITY) {
-      const float e = expf(d);
-      s += e;
-      s1 = fmaf(e, d, s1);
+  // value e of thread tid: id base + (e / 4 * LP_THREADS + tid) * 4 + e % 4
+  auto id_of = [&](int e) { return base + (e / 4 * LP_THREADS + tid) * 4 + e % 4; };
+  float v[E];
+#pragma unroll
+  for (int e = 0; e < E; e += 4) {
+    const int id = id_of(e);
+    if (VEC && id + 3 < a.vocab) {
+      const float4 f = __ldcs(reinterpret_cast<const float4*>(x + id));
+      v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[e + i] = id + i < a.vocab ? x[id + i] : -INFINITY;
     }
-    before += logit_key(v, i) > kt;
   }
-  s = warp_sum(s);
-  s1 = warp_sum(s1);
+  // this thread's largest value (NaNs left out)
+  float tm = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) tm = fmaxf(fmaxf(tm, v[e]), v[e + 1]);
+  float m = warp_max(tm);
+  if (lane == 0) redm[warp] = m;
+  if (tid == 0) {
+    count = 0;
+    lohi[0] = ~0ull;
+    lohi[1] = 0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NWARP; ++w) m = fmaxf(m, redm[w]);
+  // a slice of nothing but -inf (and NaN) is taken relative to 0
+  const float mm = m == -INFINITY ? 0.0f : m;
+  // tokens before the target: ids below it from xt on, ids above it beyond xt
+  int before = 0;
+  if (has_t) {
+    if (base > t || base + LP_THREADS * E <= t) {
+      const bool eq = base < t;
+#pragma unroll
+      for (int e = 0; e < E; ++e) before += v[e] > xt || (eq && v[e] == xt);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) before += v[e] > xt || (v[e] == xt && id_of(e) < t);
+    }
+    // (values past the vocabulary are -inf, with ids beyond the target's)
+  }
+  unsigned long long s2 = 0ull, t2 = 0ull;  // pairs: sums of p, of p d
+  const unsigned long long nm2 = pk2(-mm, -mm), l2e = pk2(1.44269504f, 1.44269504f);
+#pragma unroll
+  for (int e = 0; e < E; e += 2) {
+    const unsigned long long d2 = add2(pk2(v[e], v[e + 1]), nm2);
+    const float2 u = upk2(mul2(d2, l2e)), d = upk2(d2);
+    const unsigned long long p2 = pk2(ex2(u.x), ex2(u.y));
+    s2 = add2(s2, p2);
+    // (p is 0 from d = -127 on; -inf times that would be NaN)
+    t2 = fma2(p2, pk2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), t2);
+  }
+  const float2 sp = upk2(s2), tp = upk2(t2);
+  const float s = warp_sum(sp.x + sp.y), s1 = warp_sum(tp.x + tp.y);
   for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
   if (lane == 0) {
     red[warp] = s;
@@ -59,35 +147,150 @@ __global__ void k_logprobs_simple(const LogprobArgs a) {
     redi[warp] = before;
   }
   __syncthreads();
-  s = 0.0f, s1 = 0.0f, before = 0;
-  for (int w = 0; w < 8; ++w) {
-    s += red[w];
-    s1 += red2[w];
-    before += redi[w];
+  LogprobRow w{m, 0.0f, 0.0f, 0};
+#pragma unroll
+  for (int i = 0; i < NWARP; ++i) {
+    w.s += red[i];
+    w.s1 += red2[i];
+    w.before += redi[i];
   }
-  const bool none = m == -INFINITY && s == 0.0f;
-  const float ls = logf(s);
-  if (tid == 0) {
-    if (a.logprob) a.logprob[r] = !has_t ? __int_as_float(0x7fc00000) : none ? -INFINITY : xt - m - ls;
-    if (a.rank) a.rank[r] = has_t ? before : -1;
-    if (a.entropy) a.entropy[r] = none ? 0.0f : ls - s1 / s;
+  const bool last = a.slices == 1;
+  if (last)
+    logprob_write(a, r, w, xt, has_t, tid);
+  else if (tid == 0)
+    a.part[(size_t)r * a.slices + blockIdx.x] =
+        make_float4(w.m, w.s, w.s1, __int_as_float(w.before));
+  if (a.k == 0) return;
+
+  bool wide = !(w.s < INFINITY);  // a NaN or +inf
+  float thr = -INFINITY;
+  bool mine = true;  // this thread holds values at or above the threshold
+  if (!wide) {
+    // thresholds as ordered integers: count(tm >= lo) >= k, count(tm >= hi) < k
+    auto key32 = [](float f) {
+      const uint32_t b = __float_as_uint(f == 0.0f ? 0.0f : f);
+      return b & 0x80000000u ? ~b : b | 0x80000000u;
+    };
+    const uint32_t best = key32(tm);
+    // from the least of the warps' largest (16 of them) down, if k allows
+    uint32_t lo = 0, hi = key32(m) + 1, step = 1u << 20;
+    for (uint32_t at = hi; lo == 0 && at > step; step <<= 1) {
+      at -= step;
+      const int c = __syncthreads_count(best >= at);
+      if (c >= a.k) lo = at;
+      else hi = at;
+      if (c >= a.k && c <= a.k + LP_SLACK) hi = lo + 1;
+    }
+    while (hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      const int c = __syncthreads_count(best >= mid);
+      if (c >= a.k) lo = mid;
+      else hi = mid;
+      if (c >= a.k && c <= a.k + LP_SLACK) break;
+    }
+    mine = best >= lo;
+    wide = __syncthreads_count(mine) > a.k + LP_SLACK;
+    thr = __uint_as_float(lo & 0x80000000u ? lo & 0x7fffffffu : ~lo);
   }
-  uint64_t last = ~0ull;
-  for (int j = 0; j < a.k; ++j) {
+  uint64_t low = 1;  // the threshold as a key
+  if (wide) {
     uint64_t best = 0;
-    for (int i = tid; i < a.vocab; i += 256) {
-      const uint64_t key = logit_key(x[i], i);
-      if (key < last && key > best) best = key;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint64_t key = id_of(e) < a.vocab ? logit_key(v[e], id_of(e)) : 0ull;
+      best = key > best ? key : best;
     }
-    for (int o = 16; o; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(0xffffffffu, best, o));
-    __syncthreads();
-    if (lane == 0) redk[warp] = best;
-    __syncthreads();
-    for (int w = 0; w < 8; ++w) best = max(best, redk[w]);
-    last = best;
-    if (tid == 0) {
-      if (a.top_ids) a.top_ids[(size_t)r * a.k + j] = key_index(best);
-      if (a.top_lp) a.top_lp[(size_t)r * a.k + j] = none ? -INFINITY : key_value(best) - m - ls;
+    uint64_t l = best ? best : ~0ull, h = best;  // (0: a thread without a value)
+    for (int o = 16; o; o >>= 1) {
+      const uint64_t l3 = __shfl_xor_sync(0xffffffffu, l, o), h3 = __shfl_xor_sync(0xffffffffu, h, o);
+      l = l3 < l ? l3 : l;
+      h = h3 > h ? h3 : h;
     }
+    if (lane == 0) {
+      atomicMin(reinterpret_cast<unsigned long long*>(&lohi[0]), (unsigned long long)l);
+      atomicMax(reinterpret_cast<unsigned long long*>(&lohi[1]), (unsigned long long)h);
+    }
+    __syncthreads();
+    uint64_t lo = lohi[0], hi = lohi[1] == ~0ull ? lohi[1] : lohi[1] + 1;
+    // (where fewer threads have a value, all are taken)
+    if (__syncthreads_count(best != 0ull) <= a.k + LP_SLACK) lo = hi = 1;
+    while (hi > lo + 1) {
+      const uint64_t mid = lo + (hi - lo) / 2;
+      const int c = __syncthreads_count(best >= mid);
+      if (c >= a.k) lo = mid;
+      else hi = mid;
+      if (c >= a.k && c <= a.k + LP_SLACK) break;
+    }
+    low = lo;
+    mine = best >= low;
+  }
+  if (mine) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (!(v[e] < thr) && id_of(e) < a.vocab) {
+        const uint64_t key = logit_key(v[e], id_of(e));
+        if (key >= low) {
+          const int at = atomicAdd(&count, 1);
+          if (at < CAP) cand[at] = key;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int n = count < CAP ? count : CAP;
+  for (int i = tid; i < n; i += LP_THREADS) {
+    const uint64_t key = cand[i];
+    int place = 0;
+    for (int j = 0; j < n; ++j) place += cand[j] > key;
+    if (place < a.k) {
+      if (last)
+        logprob_top(a, r, w, key, place);
+      else
+        a.part_k[((size_t)r * a.slices + blockIdx.x) * a.k + place] = key;
+    }
+  }
+  if (!last)  // a slice of fewer than k values
+    for (int i = n + tid; i < a.k; i += LP_THREADS)
+      a.part_k[((size_t)r * a.slices + blockIdx.x) * a.k + i] = 0ull;
+}
+
+// Joins a row's slices, in their order; a key's place is the number of larger
+// ones in the slices' sorted lists.  grid rows, 128 threads.
+static __global__ void __launch_bounds__(128) k_logprobs_join(const LogprobArgs a) {
+  const int r = blockIdx.x, tid = threadIdx.x;
+  pdl_wait();
+  const float4* part = a.part + (size_t)r * a.slices;
+  const int t = a.targets ? a.targets[r] : -1;
+  const bool has_t = t >= 0 && t < a.vocab;
+  const float xt = has_t ? a.x[(long long)r * a.ld + t] : 0.0f;
+  LogprobRow w{-INFINITY, 0.0f, 0.0f, 0};
+  for (int i = 0; i < a.slices; ++i) w.m = fmaxf(w.m, part[i].x);
+  for (int i = 0; i < a.slices; ++i) {
+    const float4 p = part[i];
+    // a slice of nothing but -inf: its sums are 0 (NaN, if it has one)
+    const float d = p.x == -INFINITY ? 0.0f : p.x - w.m;
+    const float f = p.x == -INFINITY ? 1.0f : ex2(d * 1.44269504f);
+    w.s = fmaf(p.y, f, w.s);
+    w.s1 = fmaf(fmaf(p.y, d, p.z), f, w.s1);
+    w.before += __float_as_int(p.w);
+  }
+  logprob_write(a, r, w, xt, has_t, tid);
+  const uint64_t* lists = a.part_k + (size_t)r * a.slices * a.k;
+  for (int i = tid; i < a.slices * a.k; i += 128) {
+    const uint64_t key = lists[i];
+    if (key == 0ull) continue;
+    int place = i % a.k;
+    for (int j = 0; j < a.slices && place < a.k; ++j) {
+      if (j == i / a.k) continue;
+      const uint64_t* l = lists + (size_t)j * a.k;
+      int lo = 0, hi = a.k;  // keys of the list above this one
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (l[mid] > key) lo = mid + 1;
+        else hi = mid;
+      }
+      place += lo;
+    }
+    if (place < a.k) logprob_top(a, r, w, key, place);
   }
 }

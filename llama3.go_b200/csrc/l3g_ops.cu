@@ -233,9 +233,29 @@ extern "C" int l3g_chunk_attn_status(l3g_chunk_attn* h, int32_t* err, int32_t* w
 struct l3g_logprobs {
   int device = 0, nsm = 1;
   int max_rows = 0, vocab = 0;
+  float4* part = nullptr;      // the slices' sums
+  uint64_t* part_k = nullptr;  // and top keys
 };
 
-extern "C" void l3g_logprobs_free(l3g_logprobs* h) { delete h; }
+extern "C" void l3g_logprobs_free(l3g_logprobs* h) {
+  if (!h) return;
+  DeviceScope scope(h->device);
+  if (h->part) cudaFree(h->part);
+  if (h->part_k) cudaFree(h->part_k);
+  delete h;
+}
+
+// Values per thread of a slice (8, 16 or 32: 4096, 8192 or 16384 values).  One
+// slice, which needs no join, where a row fits into 8192 values; else the
+// largest slices that still give every SM two CTAs.  Measured at 128256 values
+// (the 8 / 16 / 32 in us): see l3g_logprobs_run.
+static int logprob_slice(const l3g_logprobs* h, int n) {
+  if (h->vocab <= 8 * LP_THREADS) return 8;
+  if (h->vocab <= 16 * LP_THREADS) return 16;
+  for (int e = 32; e > 8; e >>= 1)
+    if ((long long)n * ((h->vocab + e * LP_THREADS - 1) / (e * LP_THREADS)) >= 2LL * h->nsm) return e;
+  return 8;
+}
 
 extern "C" int l3g_logprobs_new(int32_t max_rows, int32_t vocab, int32_t device,
                                 l3g_logprobs** out) {
@@ -251,6 +271,18 @@ extern "C" int l3g_logprobs_new(int32_t max_rows, int32_t vocab, int32_t device,
   h->nsm = sm_count(dev);
   h->max_rows = max_rows;
   h->vocab = vocab;
+  size_t parts = 0;  // the most slices that any number of rows gets
+  for (int n = 1; n <= max_rows; n = n < 4 * h->nsm ? n + 1 : max_rows > n ? max_rows : n + 1) {
+    const int per = logprob_slice(h, n) * LP_THREADS;
+    parts = std::max(parts, (size_t)n * ((vocab + per - 1) / per));
+  }
+  cudaError_t e = cudaMalloc(&h->part, parts * sizeof(float4));
+  if (e == cudaSuccess)
+    e = cudaMalloc(&h->part_k, parts * std::min(MAX_TOPK, vocab) * sizeof(uint64_t));
+  if (e != cudaSuccess) {
+    l3g_logprobs_free(h);
+    return l3g_fail(L3G_E_CUDA, "log probabilities: %s", cudaGetErrorString(e));
+  }
   *out = h;
   return L3G_OK;
 }
@@ -288,8 +320,48 @@ extern "C" int l3g_logprobs_run(l3g_logprobs* h, const float* logits, int64_t ld
   a.rank = rank;
   a.top_ids = top_ids;
   a.top_lp = top_logprobs;
-  k_logprobs_simple<<<n, 256, 0, (cudaStream_t)stream>>>(a);
-  CUDA_TRY(cudaGetLastError());
+  const int e = logprob_slice(h, n);
+  a.slices = (h->vocab + e * LP_THREADS - 1) / (e * LP_THREADS);
+  a.part = h->part;
+  a.part_k = h->part_k;
+  const bool vec = !misaligned(logits, 16) && ld % 4 == 0;
+  const cudaStream_t st = (cudaStream_t)stream;
+  for (int r0 = 0; r0 < n; r0 += 65535) {  // rows are the grid's y
+    LogprobArgs b = a;
+    const int rows = std::min(65535, n - r0);
+    b.n = rows;
+    b.x += (long long)r0 * ld;
+    if (b.targets) b.targets += r0;
+    if (b.logprob) b.logprob += r0;
+    if (b.entropy) b.entropy += r0;
+    if (b.rank) b.rank += r0;
+    if (b.top_ids) b.top_ids += (size_t)r0 * top_k;
+    if (b.top_lp) b.top_lp += (size_t)r0 * top_k;
+    b.part += (size_t)r0 * a.slices;
+    b.part_k += (size_t)r0 * a.slices * top_k;
+    const dim3 grid(a.slices, rows);
+    switch (e * 2 + (vec ? 1 : 0)) {
+      case 16: k_logprobs_part<8, false><<<grid, LP_THREADS, 0, st>>>(b); break;
+      case 17: k_logprobs_part<8, true><<<grid, LP_THREADS, 0, st>>>(b); break;
+      case 32: k_logprobs_part<16, false><<<grid, LP_THREADS, 0, st>>>(b); break;
+      case 33: k_logprobs_part<16, true><<<grid, LP_THREADS, 0, st>>>(b); break;
+      case 64: k_logprobs_part<32, false><<<grid, LP_THREADS, 0, st>>>(b); break;
+      default: k_logprobs_part<32, true><<<grid, LP_THREADS, 0, st>>>(b); break;
+    }
+    CUDA_TRY(cudaGetLastError());
+    if (a.slices > 1) {  // launched early: it waits for the slices itself
+      cudaLaunchAttribute at{};
+      at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      at.val.programmaticStreamSerializationAllowed = 1;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(rows);
+      cfg.blockDim = dim3(128);
+      cfg.stream = st;
+      cfg.attrs = &at;
+      cfg.numAttrs = 1;
+      CUDA_TRY(cudaLaunchKernelEx(&cfg, k_logprobs_join, b));
+    }
+  }
   return L3G_OK;
 }
 
