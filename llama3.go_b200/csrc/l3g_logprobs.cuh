@@ -76,6 +76,7 @@ __global__ void __launch_bounds__(LP_THREADS, E == 32 ? 2 : 3)
   constexpr int CAP = (MAX_TOPK + LP_SLACK) * E;
   __shared__ float red[NWARP], red2[NWARP], redm[NWARP];
   __shared__ int redi[NWARP], count;
+  __shared__ uint32_t best_of[LP_THREADS], low32, ties;
   __shared__ uint64_t lohi[2], cand[CAP];
   const int r = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int base = blockIdx.x * LP_THREADS * E;
@@ -116,15 +117,9 @@ __global__ void __launch_bounds__(LP_THREADS, E == 32 ? 2 : 3)
   const float mm = m == -INFINITY ? 0.0f : m;
   // tokens before the target: ids below it from xt on, ids above it beyond xt
   int before = 0;
-  if (has_t) {
-    if (base > t || base + LP_THREADS * E <= t) {
-      const bool eq = base < t;
+  if (has_t && tm >= xt) {  // (few threads hold a value beyond a likely token's)
 #pragma unroll
-      for (int e = 0; e < E; ++e) before += v[e] > xt || (eq && v[e] == xt);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) before += v[e] > xt || (v[e] == xt && id_of(e) < t);
-    }
+    for (int e = 0; e < E; ++e) before += v[e] > xt || (v[e] == xt && id_of(e) < t);
     // (values past the vocabulary are -inf, with ids beyond the target's)
   }
   unsigned long long s2 = 0ull, t2 = 0ull;  // pairs: sums of p, of p d
@@ -166,30 +161,50 @@ __global__ void __launch_bounds__(LP_THREADS, E == 32 ? 2 : 3)
   float thr = -INFINITY;
   bool mine = true;  // this thread holds values at or above the threshold
   if (!wide) {
-    // thresholds as ordered integers: count(tm >= lo) >= k, count(tm >= hi) < k
+    // the threshold as an ordered integer, by warp 0 from all threads' values:
+    // count(tm >= lo) >= k, count(tm >= hi) < k
     auto key32 = [](float f) {
       const uint32_t b = __float_as_uint(f == 0.0f ? 0.0f : f);
       return b & 0x80000000u ? ~b : b | 0x80000000u;
     };
     const uint32_t best = key32(tm);
-    // from the least of the warps' largest (16 of them) down, if k allows
-    uint32_t lo = 0, hi = key32(m) + 1, step = 1u << 20;
-    for (uint32_t at = hi; lo == 0 && at > step; step <<= 1) {
-      at -= step;
-      const int c = __syncthreads_count(best >= at);
-      if (c >= a.k) lo = at;
-      else hi = at;
-      if (c >= a.k && c <= a.k + LP_SLACK) hi = lo + 1;
+    best_of[tid] = best;
+    __syncthreads();
+    if (warp == 0) {
+      uint32_t b[NWARP];
+#pragma unroll
+      for (int i = 0; i < NWARP; ++i) b[i] = best_of[i * 32 + lane];
+      auto at_least = [&](uint32_t k32) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < NWARP; ++i) c += b[i] >= k32;
+        return (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
+      };
+      // steps down from the largest, doubling, then halves
+      uint32_t lo = 0, hi = key32(m) + 1, step = 1u << 20;
+      int c = 0, at_lo = LP_THREADS;  // threads at or above lo
+      while (lo == 0 && hi > step) {
+        const uint32_t at = hi - step;
+        step <<= 1;
+        c = at_least(at);
+        if (c >= a.k) lo = at, at_lo = c;
+        else hi = at;
+      }
+      while (hi - lo > 1 && at_lo > a.k + LP_SLACK) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        c = at_least(mid);
+        if (c >= a.k) lo = mid, at_lo = c;
+        else hi = mid;
+      }
+      if (lane == 0) {
+        low32 = lo;
+        ties = at_lo > a.k + LP_SLACK;
+      }
     }
-    while (hi - lo > 1) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      const int c = __syncthreads_count(best >= mid);
-      if (c >= a.k) lo = mid;
-      else hi = mid;
-      if (c >= a.k && c <= a.k + LP_SLACK) break;
-    }
+    __syncthreads();
+    const uint32_t lo = low32;
     mine = best >= lo;
-    wide = __syncthreads_count(mine) > a.k + LP_SLACK;
+    wide = ties;
     thr = __uint_as_float(lo & 0x80000000u ? lo & 0x7fffffffu : ~lo);
   }
   uint64_t low = 1;  // the threshold as a key
@@ -225,10 +240,16 @@ __global__ void __launch_bounds__(LP_THREADS, E == 32 ? 2 : 3)
     mine = best >= low;
   }
   if (mine) {
+    // the places of its values at or above the threshold, then those one by one
+    uint32_t set = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (!(v[e] < thr) && id_of(e) < a.vocab) {
-        const uint64_t key = logit_key(v[e], id_of(e));
+    for (int e = 0; e < E; ++e) set |= (v[e] < thr ? 0u : 1u) << e;
+    while (set) {
+      const int e = __ffs(set) - 1;
+      set &= set - 1;
+      const int id = id_of(e);
+      if (id < a.vocab) {
+        const uint64_t key = logit_key(x[id], id);  // (read again: no registers by index)
         if (key >= low) {
           const int at = atomicAdd(&count, 1);
           if (at < CAP) cand[at] = key;
@@ -241,6 +262,7 @@ __global__ void __launch_bounds__(LP_THREADS, E == 32 ? 2 : 3)
   for (int i = tid; i < n; i += LP_THREADS) {
     const uint64_t key = cand[i];
     int place = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) place += cand[j] > key;
     if (place < a.k) {
       if (last)
@@ -254,35 +276,66 @@ __global__ void __launch_bounds__(LP_THREADS, E == 32 ? 2 : 3)
       a.part_k[((size_t)r * a.slices + blockIdx.x) * a.k + i] = 0ull;
 }
 
-// Joins a row's slices, in their order; a key's place is the number of larger
-// ones in the slices' sorted lists.  grid rows, 128 threads.
-static __global__ void __launch_bounds__(128) k_logprobs_join(const LogprobArgs a) {
+// Joins a row's slices; a key's place is the number of larger ones in the
+// slices' sorted lists: of all keys where there are few, else by searching the
+// lists, in shared memory where they fit.  grid rows.
+constexpr int LP_JOIN = 256, LP_LISTS = 2048, LP_PAIRS = 1024;
+static __global__ void __launch_bounds__(LP_JOIN) k_logprobs_join(const LogprobArgs a) {
+  __shared__ uint64_t keys[LP_LISTS];
+  __shared__ float4 sums;
   const int r = blockIdx.x, tid = threadIdx.x;
-  pdl_wait();
-  const float4* part = a.part + (size_t)r * a.slices;
   const int t = a.targets ? a.targets[r] : -1;
   const bool has_t = t >= 0 && t < a.vocab;
   const float xt = has_t ? a.x[(long long)r * a.ld + t] : 0.0f;
-  LogprobRow w{-INFINITY, 0.0f, 0.0f, 0};
-  for (int i = 0; i < a.slices; ++i) w.m = fmaxf(w.m, part[i].x);
-  for (int i = 0; i < a.slices; ++i) {
-    const float4 p = part[i];
-    // a slice of nothing but -inf: its sums are 0 (NaN, if it has one)
-    const float d = p.x == -INFINITY ? 0.0f : p.x - w.m;
-    const float f = p.x == -INFINITY ? 1.0f : ex2(d * 1.44269504f);
-    w.s = fmaf(p.y, f, w.s);
-    w.s1 = fmaf(fmaf(p.y, d, p.z), f, w.s1);
-    w.before += __float_as_int(p.w);
+  const int n = a.slices * a.k;
+  pdl_wait();
+  const float4* part = a.part + (size_t)r * a.slices;
+  const uint64_t* lists = a.part_k + (size_t)r * n;
+  if (tid < 32) {  // a lane the slices lane, lane + 32 ..; then a tree over lanes
+    float m = -INFINITY;
+    for (int i = tid; i < a.slices; i += 32) m = fmaxf(m, part[i].x);
+    m = warp_max(m);
+    float s = 0.0f, s1 = 0.0f;
+    int before = 0;
+    for (int i = tid; i < a.slices; i += 32) {
+      const float4 p = part[i];
+      // a slice of nothing but -inf: its sums are 0 (NaN, if it has one)
+      const float d = p.x == -INFINITY ? 0.0f : p.x - m;
+      const float f = p.x == -INFINITY ? 1.0f : ex2(d * 1.44269504f);
+      s = fmaf(p.y, f, s);
+      s1 = fmaf(fmaf(p.y, d, p.z), f, s1);
+      before += __float_as_int(p.w);
+    }
+    s = warp_sum(s);
+    s1 = warp_sum(s1);
+    for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    if (tid == 0) sums = make_float4(m, s, s1, __int_as_float(before));
   }
+  const bool fit = n <= LP_LISTS;
+  if (fit)
+    for (int i = tid; i < n; i += LP_JOIN) keys[i] = lists[i];
+  __syncthreads();
+  const LogprobRow w{sums.x, sums.y, sums.z, __float_as_int(sums.w)};
   logprob_write(a, r, w, xt, has_t, tid);
-  const uint64_t* lists = a.part_k + (size_t)r * a.slices * a.k;
-  for (int i = tid; i < a.slices * a.k; i += 128) {
-    const uint64_t key = lists[i];
+  if (n <= LP_PAIRS) {  // few keys: against every other one
+    for (int i = tid; i < n; i += LP_JOIN) {
+      const uint64_t key = keys[i];
+      int place = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) place += keys[j] > key;
+      if (key != 0ull && place < a.k) logprob_top(a, r, w, key, place);
+    }
+    return;
+  }
+  const uint64_t* from = fit ? keys : lists;
+  for (int i = tid; i < n; i += LP_JOIN) {
+    const uint64_t key = from[i];
     if (key == 0ull) continue;
+    const int own = i / a.k;
     int place = i % a.k;
     for (int j = 0; j < a.slices && place < a.k; ++j) {
-      if (j == i / a.k) continue;
-      const uint64_t* l = lists + (size_t)j * a.k;
+      if (j == own) continue;
+      const uint64_t* l = from + (size_t)j * a.k;
       int lo = 0, hi = a.k;  // keys of the list above this one
       while (lo < hi) {
         const int mid = (lo + hi) / 2;

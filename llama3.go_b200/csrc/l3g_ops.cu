@@ -355,7 +355,7 @@ extern "C" int l3g_logprobs_run(l3g_logprobs* h, const float* logits, int64_t ld
       at.val.programmaticStreamSerializationAllowed = 1;
       cudaLaunchConfig_t cfg{};
       cfg.gridDim = dim3(rows);
-      cfg.blockDim = dim3(128);
+      cfg.blockDim = dim3(LP_JOIN);
       cfg.stream = st;
       cfg.attrs = &at;
       cfg.numAttrs = 1;
