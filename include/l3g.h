@@ -542,6 +542,8 @@ int l3g_logprobs_run(l3g_logprobs *h, const float *logits, int64_t ld,
                      int32_t n, const int32_t *targets, float *logprob,
                      float *entropy, int32_t *rank, int32_t top_k,
                      int32_t *top_ids, float *top_logprobs, void *stream);
+/* As l3g_chunk_attn_status (err 0 or 1). */
+int l3g_logprobs_status(l3g_logprobs *h, int32_t *err, int32_t *where);
 
 /* Copies rows between pages: for i < n the first rows[i] rows (rows NULL: all
  * L3G_KV_PAGE) of page src[i] of src_pool to page dst[i] of dst_pool; a page is

@@ -9,7 +9,8 @@
 // The pass is bound by memory: 4 bytes and about 16 instructions a value.
 #pragma once
 
-constexpr int LP_THREADS = 512;
+constexpr int LP_THREADS = 256;
+constexpr int LP_CAND = 1024;  // gathered keys
 // Threads with a key at or above the threshold that the search stops at: k and
 // up to LP_SLACK more.
 constexpr int LP_SLACK = 16;
@@ -24,6 +25,8 @@ struct LogprobArgs {
   int* rank;
   int* top_ids;
   float* top_lp;
+  Result* res;
+  unsigned long long wait_ns;
   float4* part;     // [n][slices] {m, S, S1, tokens before the target (bits)}
   uint64_t* part_k; // [n][slices][k] the slices' top keys, sorted
 };
@@ -57,123 +60,170 @@ __device__ __forceinline__ void logprob_top(const LogprobArgs& a, int r, const L
     a.top_lp[(size_t)r * a.k + place] = none ? -INFINITY : key_value(key) - w.m - logf(w.s);
 }
 
-// One slice of LP_THREADS * E values.  grid (slices, rows).  VEC: rows start on
-// 16-byte boundaries.
+// Slices of LP_THREADS * E values, dealt to as many CTAs as fit at once.  VEC:
+// rows start on 16-byte boundaries; a slice then comes by one bulk copy into
+// shared memory while the slice before is worked on, so that memory is never
+// idle: a slice's chain of barriers (maximum, sums and threshold, candidates)
+// takes longer than its bytes need.  Few threads with many values each: what a
+// thread does once per slice costs as much as its values.
 //
 // The top k of the slice: the k-th largest of the threads' own largest values
 // is at or below the slice's k-th value, so every one of the top k belongs to a
-// thread whose largest is at or above it.  That threshold is bisected, on the
-// values' bits, until k to k + LP_SLACK threads are at or above it; their at
-// most (k + LP_SLACK) * E values at or above it are gathered as keys (value and
-// id) and each finds its place by counting the larger ones.  The work hardly
-// depends on the values: a descending row costs what a random one does.  Where
-// too many threads tie, or the slice holds a NaN or +inf, whole keys, which all
-// differ, are bisected instead.
+// thread whose largest is at or above it.  One warp bisects that threshold, on
+// the values' bits, until k to k + LP_SLACK threads are at or above it; their
+// values at or above it are gathered as keys (value and id) and each finds its
+// place by counting the larger ones.  The work hardly depends on the values: a
+// descending row costs what a random one does.  Where too many threads tie, too
+// many values are at or above the threshold, or the slice holds a NaN or +inf,
+// the k keys are found one by one.
+constexpr int lp_smem(int e) { return 2 * LP_THREADS * e * 4; }
 template <int E, bool VEC>
-__global__ void __launch_bounds__(LP_THREADS, E == 32 ? 2 : 3)
-    k_logprobs_part(const LogprobArgs a) {
+__global__ void __launch_bounds__(LP_THREADS, 3) k_logprobs_part(const LogprobArgs a) {
   constexpr int NWARP = LP_THREADS / 32;
-  constexpr int CAP = (MAX_TOPK + LP_SLACK) * E;
-  __shared__ float red[NWARP], red2[NWARP], redm[NWARP];
+  constexpr int SLICE = LP_THREADS * E;
+  __shared__ uint64_t full[2];
+  __shared__ int abort_flag;
+  __shared__ float red[NWARP], red2[NWARP], redm[NWARP], best_of[LP_THREADS];
   __shared__ int redi[NWARP], count;
-  __shared__ uint32_t best_of[LP_THREADS], low32, ties;
-  __shared__ uint64_t lohi[2], cand[CAP];
-  const int r = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int base = blockIdx.x * LP_THREADS * E;
-  const float* x = a.x + (long long)r * a.ld;
+  __shared__ uint32_t low32, slow;
+  __shared__ uint64_t cand[LP_CAND];
+  L3G_DYNAMIC_SMEM(lp_buf);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
-  const int t = a.targets ? a.targets[r] : -1;
-  const bool has_t = t >= 0 && t < a.vocab;
-  const float xt = has_t ? x[t] : 0.0f;
-  // value e of thread tid: id base + (e / 4 * LP_THREADS + tid) * 4 + e % 4
-  auto id_of = [&](int e) { return base + (e / 4 * LP_THREADS + tid) * 4 + e % 4; };
-  float v[E];
-#pragma unroll
-  for (int e = 0; e < E; e += 4) {
-    const int id = id_of(e);
-    if (VEC && id + 3 < a.vocab) {
-      const float4 f = __ldcs(reinterpret_cast<const float4*>(x + id));
-      v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[e + i] = id + i < a.vocab ? x[id + i] : -INFINITY;
+  const unsigned total = (unsigned)a.n * a.slices;  // (max_rows x slices is below 2^31)
+  // thread 0: the copy of the CTA's i-th slice
+  auto fetch = [&](int i) {
+    const unsigned at = blockIdx.x + i * gridDim.x;
+    if (at >= total) return;
+    const unsigned row = at / a.slices;
+    const int base = (int)(at - row * a.slices) * SLICE;
+    const int cnt = a.vocab - base < SLICE ? a.vocab - base : SLICE;
+    const uint32_t bytes = (uint32_t)(cnt & ~3) * 4;  // the last values are read as they are
+    mbar_arrive_expect_tx(&full[i & 1], bytes);
+    if (bytes)
+      bulk_g2s(lp_buf + (size_t)(i & 1) * SLICE * 4, a.x + (long long)row * a.ld + base, bytes,
+               &full[i & 1]);
+  };
+  if (VEC && tid == 0) {
+    mbar_init(&full[0], 1);
+    mbar_init(&full[1], 1);
+    abort_flag = 0;
+    fence_mbar_init();
+    fetch(0);
+  }
+  // the row's target and its logit, a slice ahead
+  auto target = [&](unsigned at) {
+    return a.targets && at < total ? a.targets[at / a.slices] : -1;
+  };
+  auto logit = [&](unsigned at, int t) {
+    return t >= 0 && t < a.vocab ? a.x[(long long)(at / a.slices) * a.ld + t] : 0.0f;
+  };
+  int t = target(blockIdx.x);
+  float xt = logit(blockIdx.x, t);
+  int round = 0;
+  for (unsigned at = blockIdx.x; at < total; at += gridDim.x, ++round) {
+    const int r = (int)(at / a.slices), slice = (int)(at - (unsigned)r * a.slices);
+    const int base = slice * SLICE;
+    const float* x = a.x + (long long)r * a.ld;
+    const bool has_t = t >= 0 && t < a.vocab;
+    const int t_next = target(at + gridDim.x);
+    // value e of thread tid: id base + (e / 4 * LP_THREADS + tid) * 4 + e % 4
+    auto id_of = [&](int e) { return base + (e / 4 * LP_THREADS + tid) * 4 + e % 4; };
+    __syncthreads();  // the slice before is done with shared memory
+    if (tid == 0) count = 0;
+    if (VEC) {
+      if (tid == 0) fetch(round + 1);
+      if (!mbar_wait(&full[round & 1], round >> 1 & 1, &abort_flag, a.res, 60, a.wait_ns))
+        abort_flag = 1;
     }
-  }
-  // this thread's largest value (NaNs left out)
-  float tm = -INFINITY;
+    const float* buf = reinterpret_cast<const float*>(lp_buf) + (size_t)(round & 1) * SLICE;
+    float v[E];
 #pragma unroll
-  for (int e = 0; e < E; e += 2) tm = fmaxf(fmaxf(tm, v[e]), v[e + 1]);
-  float m = warp_max(tm);
-  if (lane == 0) redm[warp] = m;
-  if (tid == 0) {
-    count = 0;
-    lohi[0] = ~0ull;
-    lohi[1] = 0;
-  }
-  __syncthreads();
+    for (int e = 0; e < E; e += 4) {
+      const int id = id_of(e);
+      if (VEC && id + 3 < a.vocab) {
+        const float4 f = *reinterpret_cast<const float4*>(buf + id - base);
+        v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
+      } else {
 #pragma unroll
-  for (int w = 0; w < NWARP; ++w) m = fmaxf(m, redm[w]);
-  // a slice of nothing but -inf (and NaN) is taken relative to 0
-  const float mm = m == -INFINITY ? 0.0f : m;
-  // tokens before the target: ids below it from xt on, ids above it beyond xt
-  int before = 0;
-  if (has_t && tm >= xt) {  // (few threads hold a value beyond a likely token's)
+        for (int i = 0; i < 4; ++i) v[e + i] = id + i < a.vocab ? x[id + i] : -INFINITY;
+      }
+    }
+    // this thread's largest value (NaNs left out)
+    float tm = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < E; ++e) before += v[e] > xt || (v[e] == xt && id_of(e) < t);
+    for (int e = 0; e < E; e += 2) tm = fmaxf(fmaxf(tm, v[e]), v[e + 1]);
+    best_of[tid] = tm;
+    const float wm = warp_max(tm);
+    if (lane == 0) redm[warp] = wm;
+    __syncthreads();
+    if (VEC && *(volatile int*)&abort_flag) return;  // (uniform: set before the barrier)
+    const float m = warp_max(redm[lane % NWARP]);
+    // a slice of nothing but -inf (and NaN) is taken relative to 0
+    const float mm = m == -INFINITY ? 0.0f : m;
+    unsigned long long s2 = 0ull, t2 = 0ull;  // pairs: sums of p, of p d
+    const unsigned long long nm2 = pk2(-mm, -mm), l2e = pk2(1.44269504f, 1.44269504f);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const unsigned long long d2 = add2(pk2(v[e], v[e + 1]), nm2);
+      const float2 u = upk2(mul2(d2, l2e)), d = upk2(d2);
+      const unsigned long long p2 = pk2(ex2(u.x), ex2(u.y));
+      s2 = add2(s2, p2);
+      // (p is 0 from d = -127 on; -inf times that would be NaN)
+      t2 = fma2(p2, pk2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), t2);
+    }
+    // tokens before the target: ids below it from xt on, ids above it beyond xt
     // (values past the vocabulary are -inf, with ids beyond the target's)
-  }
-  unsigned long long s2 = 0ull, t2 = 0ull;  // pairs: sums of p, of p d
-  const unsigned long long nm2 = pk2(-mm, -mm), l2e = pk2(1.44269504f, 1.44269504f);
+    int before = 0;
+    if (has_t && tm >= xt) {  // (few threads hold a value beyond a likely token's)
+      if (base > t) {
 #pragma unroll
-  for (int e = 0; e < E; e += 2) {
-    const unsigned long long d2 = add2(pk2(v[e], v[e + 1]), nm2);
-    const float2 u = upk2(mul2(d2, l2e)), d = upk2(d2);
-    const unsigned long long p2 = pk2(ex2(u.x), ex2(u.y));
-    s2 = add2(s2, p2);
-    // (p is 0 from d = -127 on; -inf times that would be NaN)
-    t2 = fma2(p2, pk2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), t2);
-  }
-  const float2 sp = upk2(s2), tp = upk2(t2);
-  const float s = warp_sum(sp.x + sp.y), s1 = warp_sum(tp.x + tp.y);
-  for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-  if (lane == 0) {
-    red[warp] = s;
-    red2[warp] = s1;
-    redi[warp] = before;
-  }
-  __syncthreads();
-  LogprobRow w{m, 0.0f, 0.0f, 0};
+        for (int e = 0; e < E; ++e) before += v[e] > xt;
+      } else if (base + SLICE <= t) {
 #pragma unroll
-  for (int i = 0; i < NWARP; ++i) {
-    w.s += red[i];
-    w.s1 += red2[i];
-    w.before += redi[i];
-  }
-  const bool last = a.slices == 1;
-  if (last)
-    logprob_write(a, r, w, xt, has_t, tid);
-  else if (tid == 0)
-    a.part[(size_t)r * a.slices + blockIdx.x] =
-        make_float4(w.m, w.s, w.s1, __int_as_float(w.before));
-  if (a.k == 0) return;
+        for (int e = 0; e < E; ++e) before += v[e] >= xt;
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) before += v[e] > xt || (v[e] == xt && id_of(e) < t);
+      }
+    }
+    const float2 sp = upk2(s2), tp = upk2(t2);
+    const float s = warp_sum(sp.x + sp.y), s1 = warp_sum(tp.x + tp.y);
+    before = (int)__reduce_add_sync(0xffffffffu, (unsigned)before);
+    if (lane == 0) {
+      red[warp] = s;
+      red2[warp] = s1;
+      redi[warp] = before;
+    }
+    const float xt_next = logit(at + gridDim.x, t_next);
+    __syncthreads();
+    LogprobRow w{m, 0.0f, 0.0f, 0};
+    const bool last = a.slices == 1;
+    if (warp == 0 || last) {
+#pragma unroll
+      for (int i = 0; i < NWARP; ++i) {
+        w.s += red[i];
+        w.s1 += red2[i];
+        w.before += redi[i];
+      }
+    }
+    if (last)
+      logprob_write(a, r, w, xt, has_t, tid);
+    else if (tid == 0)
+      a.part[(size_t)r * a.slices + slice] = make_float4(w.m, w.s, w.s1, __int_as_float(w.before));
+    t = t_next;
+    xt = xt_next;
+    if (a.k == 0) continue;
 
-  bool wide = !(w.s < INFINITY);  // a NaN or +inf
-  float thr = -INFINITY;
-  bool mine = true;  // this thread holds values at or above the threshold
-  if (!wide) {
-    // the threshold as an ordered integer, by warp 0 from all threads' values:
-    // count(tm >= lo) >= k, count(tm >= hi) < k
+    // the threshold as an ordered integer: count(tm >= lo) >= k, count(tm >= hi) < k
     auto key32 = [](float f) {
       const uint32_t b = __float_as_uint(f == 0.0f ? 0.0f : f);
       return b & 0x80000000u ? ~b : b | 0x80000000u;
     };
-    const uint32_t best = key32(tm);
-    best_of[tid] = best;
-    __syncthreads();
     if (warp == 0) {
       uint32_t b[NWARP];
 #pragma unroll
-      for (int i = 0; i < NWARP; ++i) b[i] = best_of[i * 32 + lane];
+      for (int i = 0; i < NWARP; ++i) b[i] = key32(best_of[i * 32 + lane]);
       auto at_least = [&](uint32_t k32) {
         int c = 0;
 #pragma unroll
@@ -184,11 +234,11 @@ __global__ void __launch_bounds__(LP_THREADS, E == 32 ? 2 : 3)
       uint32_t lo = 0, hi = key32(m) + 1, step = 1u << 20;
       int c = 0, at_lo = LP_THREADS;  // threads at or above lo
       while (lo == 0 && hi > step) {
-        const uint32_t at = hi - step;
+        const uint32_t mid = hi - step;
         step <<= 1;
-        c = at_least(at);
-        if (c >= a.k) lo = at, at_lo = c;
-        else hi = at;
+        c = at_least(mid);
+        if (c >= a.k) lo = mid, at_lo = c;
+        else hi = mid;
       }
       while (hi - lo > 1 && at_lo > a.k + LP_SLACK) {
         const uint32_t mid = lo + (hi - lo) / 2;
@@ -198,82 +248,67 @@ __global__ void __launch_bounds__(LP_THREADS, E == 32 ? 2 : 3)
       }
       if (lane == 0) {
         low32 = lo;
-        ties = at_lo > a.k + LP_SLACK;
+        slow = at_lo > a.k + LP_SLACK || !(w.s < INFINITY);
       }
     }
     __syncthreads();
-    const uint32_t lo = low32;
-    mine = best >= lo;
-    wide = ties;
-    thr = __uint_as_float(lo & 0x80000000u ? lo & 0x7fffffffu : ~lo);
-  }
-  uint64_t low = 1;  // the threshold as a key
-  if (wide) {
-    uint64_t best = 0;
+    if (!slow && key32(tm) >= low32) {
+      // the places of its values at or above the threshold, then those one by one
+      const float thr = __uint_as_float(low32 & 0x80000000u ? low32 & 0x7fffffffu : ~low32);
+      uint32_t set = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const uint64_t key = id_of(e) < a.vocab ? logit_key(v[e], id_of(e)) : 0ull;
-      best = key > best ? key : best;
-    }
-    uint64_t l = best ? best : ~0ull, h = best;  // (0: a thread without a value)
-    for (int o = 16; o; o >>= 1) {
-      const uint64_t l3 = __shfl_xor_sync(0xffffffffu, l, o), h3 = __shfl_xor_sync(0xffffffffu, h, o);
-      l = l3 < l ? l3 : l;
-      h = h3 > h ? h3 : h;
-    }
-    if (lane == 0) {
-      atomicMin(reinterpret_cast<unsigned long long*>(&lohi[0]), (unsigned long long)l);
-      atomicMax(reinterpret_cast<unsigned long long*>(&lohi[1]), (unsigned long long)h);
-    }
-    __syncthreads();
-    uint64_t lo = lohi[0], hi = lohi[1] == ~0ull ? lohi[1] : lohi[1] + 1;
-    // (where fewer threads have a value, all are taken)
-    if (__syncthreads_count(best != 0ull) <= a.k + LP_SLACK) lo = hi = 1;
-    while (hi > lo + 1) {
-      const uint64_t mid = lo + (hi - lo) / 2;
-      const int c = __syncthreads_count(best >= mid);
-      if (c >= a.k) lo = mid;
-      else hi = mid;
-      if (c >= a.k && c <= a.k + LP_SLACK) break;
-    }
-    low = lo;
-    mine = best >= low;
-  }
-  if (mine) {
-    // the places of its values at or above the threshold, then those one by one
-    uint32_t set = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) set |= (v[e] < thr ? 0u : 1u) << e;
-    while (set) {
-      const int e = __ffs(set) - 1;
-      set &= set - 1;
-      const int id = id_of(e);
-      if (id < a.vocab) {
-        const uint64_t key = logit_key(x[id], id);  // (read again: no registers by index)
-        if (key >= low) {
-          const int at = atomicAdd(&count, 1);
-          if (at < CAP) cand[at] = key;
+      for (int e = 0; e < E; ++e) set |= (v[e] < thr ? 0u : 1u) << e;
+      while (set) {
+        const int e = __ffs(set) - 1;
+        set &= set - 1;
+        const int id = id_of(e);
+        if (id < a.vocab) {
+          // (read again: no registers by index)
+          const uint64_t key = logit_key(VEC && (id | 3) < a.vocab ? buf[id - base] : x[id], id);
+          const int place = atomicAdd(&count, 1);
+          if (place < LP_CAND) cand[place] = key;
         }
       }
     }
-  }
-  __syncthreads();
-  const int n = count < CAP ? count : CAP;
-  for (int i = tid; i < n; i += LP_THREADS) {
-    const uint64_t key = cand[i];
-    int place = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) place += cand[j] > key;
-    if (place < a.k) {
-      if (last)
-        logprob_top(a, r, w, key, place);
-      else
-        a.part_k[((size_t)r * a.slices + blockIdx.x) * a.k + place] = key;
+    __syncthreads();
+    int n = count;
+    if (slow || n > LP_CAND) {  // one by one: the largest key below the last
+      n = 0;
+      uint64_t below = ~0ull;
+      bool first = true;
+      for (; n < a.k; ++n) {
+        uint64_t best = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const uint64_t key = id_of(e) < a.vocab ? logit_key(v[e], id_of(e)) : 0ull;
+          if ((key < below || first) && key > best) best = key;
+        }
+        __syncthreads();  // cand[n] is not yet in use, or was cleared by all
+        if (tid == 0) cand[n] = 0ull;
+        __syncthreads();
+        atomicMax(reinterpret_cast<unsigned long long*>(&cand[n]), (unsigned long long)best);
+        __syncthreads();
+        below = cand[n];
+        first = false;
+        if (below == 0ull) break;  // no values left
+      }
     }
+    for (int i = tid; i < n; i += LP_THREADS) {
+      const uint64_t key = cand[i];
+      int place = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) place += cand[j] > key;
+      if (place < a.k) {
+        if (last)
+          logprob_top(a, r, w, key, place);
+        else
+          a.part_k[((size_t)r * a.slices + slice) * a.k + place] = key;
+      }
+    }
+    if (!last)  // a slice of fewer than k values
+      for (int i = n + tid; i < a.k; i += LP_THREADS)
+        a.part_k[((size_t)r * a.slices + slice) * a.k + i] = 0ull;
   }
-  if (!last)  // a slice of fewer than k values
-    for (int i = n + tid; i < a.k; i += LP_THREADS)
-      a.part_k[((size_t)r * a.slices + blockIdx.x) * a.k + i] = 0ull;
 }
 
 // Joins a row's slices; a key's place is the number of larger ones in the

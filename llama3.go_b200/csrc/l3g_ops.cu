@@ -235,6 +235,7 @@ struct l3g_logprobs {
   int max_rows = 0, vocab = 0;
   float4* part = nullptr;      // the slices' sums
   uint64_t* part_k = nullptr;  // and top keys
+  Result* d_res = nullptr;     // device error word of the kernel's bounded waits
 };
 
 extern "C" void l3g_logprobs_free(l3g_logprobs* h) {
@@ -242,19 +243,39 @@ extern "C" void l3g_logprobs_free(l3g_logprobs* h) {
   DeviceScope scope(h->device);
   if (h->part) cudaFree(h->part);
   if (h->part_k) cudaFree(h->part_k);
+  if (h->d_res) cudaFree(h->d_res);
   delete h;
 }
 
-// Values per thread of a slice (8, 16 or 32: 4096, 8192 or 16384 values).  One
-// slice, which needs no join, where a row fits into 8192 values; else the
-// largest slices that still give every SM two CTAs.  Measured at 128256 values
-// (the 8 / 16 / 32 in us): see l3g_logprobs_run.
+// Values per thread of a slice (16 or 32: 4096 or 8192 values): the larger ones
+// where a row then needs no join, or where they still fill the CTAs that fit at
+// once (three per SM).
 static int logprob_slice(const l3g_logprobs* h, int n) {
-  if (h->vocab <= 8 * LP_THREADS) return 8;
+  const int big = 32 * LP_THREADS;
   if (h->vocab <= 16 * LP_THREADS) return 16;
-  for (int e = 32; e > 8; e >>= 1)
-    if ((long long)n * ((h->vocab + e * LP_THREADS - 1) / (e * LP_THREADS)) >= 2LL * h->nsm) return e;
-  return 8;
+  if (h->vocab <= big) return 32;
+  return (long long)n * ((h->vocab + big - 1) / big) >= 3LL * h->nsm ? 32 : 16;
+}
+
+// Kernel attributes, once per device, with that device current.
+static int logprob_setup() {
+  static int rcs[64];
+  static std::once_flag onces[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
+    return l3g_fail(L3G_E_CUDA, "log probabilities set-up: no current device");
+  int& rc = rcs[dev];
+  std::call_once(onces[dev], [&rc] {
+    cudaError_t e = cudaFuncSetAttribute(
+        k_logprobs_part<16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, lp_smem(16));
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(k_logprobs_part<32, true>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, lp_smem(32));
+    rc = e == cudaSuccess ? L3G_OK
+                          : l3g_fail(L3G_E_CUDA, "log probabilities attributes: %s",
+                                     cudaGetErrorString(e));
+  });
+  return rc ? l3g_fail(L3G_E_CUDA, "log probabilities set-up failed on device %d", dev) : L3G_OK;
 }
 
 extern "C" int l3g_logprobs_new(int32_t max_rows, int32_t vocab, int32_t device,
@@ -266,6 +287,7 @@ extern "C" int l3g_logprobs_new(int32_t max_rows, int32_t vocab, int32_t device,
   int dev = device;
   if (dev < 0) CUDA_TRY(cudaGetDevice(&dev));
   ON_DEVICE(dev);
+  if (int rc = logprob_setup()) return rc;
   auto* h = new l3g_logprobs();
   h->device = dev;
   h->nsm = sm_count(dev);
@@ -279,6 +301,8 @@ extern "C" int l3g_logprobs_new(int32_t max_rows, int32_t vocab, int32_t device,
   cudaError_t e = cudaMalloc(&h->part, parts * sizeof(float4));
   if (e == cudaSuccess)
     e = cudaMalloc(&h->part_k, parts * std::min(MAX_TOPK, vocab) * sizeof(uint64_t));
+  if (e == cudaSuccess) e = cudaMalloc(&h->d_res, sizeof(Result));
+  if (e == cudaSuccess) e = cudaMemset(h->d_res, 0, sizeof(Result));
   if (e != cudaSuccess) {
     l3g_logprobs_free(h);
     return l3g_fail(L3G_E_CUDA, "log probabilities: %s", cudaGetErrorString(e));
@@ -326,42 +350,39 @@ extern "C" int l3g_logprobs_run(l3g_logprobs* h, const float* logits, int64_t ld
   a.part_k = h->part_k;
   const bool vec = !misaligned(logits, 16) && ld % 4 == 0;
   const cudaStream_t st = (cudaStream_t)stream;
-  for (int r0 = 0; r0 < n; r0 += 65535) {  // rows are the grid's y
-    LogprobArgs b = a;
-    const int rows = std::min(65535, n - r0);
-    b.n = rows;
-    b.x += (long long)r0 * ld;
-    if (b.targets) b.targets += r0;
-    if (b.logprob) b.logprob += r0;
-    if (b.entropy) b.entropy += r0;
-    if (b.rank) b.rank += r0;
-    if (b.top_ids) b.top_ids += (size_t)r0 * top_k;
-    if (b.top_lp) b.top_lp += (size_t)r0 * top_k;
-    b.part += (size_t)r0 * a.slices;
-    b.part_k += (size_t)r0 * a.slices * top_k;
-    const dim3 grid(a.slices, rows);
-    switch (e * 2 + (vec ? 1 : 0)) {
-      case 16: k_logprobs_part<8, false><<<grid, LP_THREADS, 0, st>>>(b); break;
-      case 17: k_logprobs_part<8, true><<<grid, LP_THREADS, 0, st>>>(b); break;
-      case 32: k_logprobs_part<16, false><<<grid, LP_THREADS, 0, st>>>(b); break;
-      case 33: k_logprobs_part<16, true><<<grid, LP_THREADS, 0, st>>>(b); break;
-      case 64: k_logprobs_part<32, false><<<grid, LP_THREADS, 0, st>>>(b); break;
-      default: k_logprobs_part<32, true><<<grid, LP_THREADS, 0, st>>>(b); break;
-    }
-    CUDA_TRY(cudaGetLastError());
-    if (a.slices > 1) {  // launched early: it waits for the slices itself
-      cudaLaunchAttribute at{};
-      at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      at.val.programmaticStreamSerializationAllowed = 1;
-      cudaLaunchConfig_t cfg{};
-      cfg.gridDim = dim3(rows);
-      cfg.blockDim = dim3(LP_JOIN);
-      cfg.stream = st;
-      cfg.attrs = &at;
-      cfg.numAttrs = 1;
-      CUDA_TRY(cudaLaunchKernelEx(&cfg, k_logprobs_join, b));
-    }
+  a.res = h->d_res;
+  a.wait_ns = WAIT_TIMEOUT_NS;
+  const int grid = (int)std::min<long long>((long long)n * a.slices, 3LL * h->nsm);
+  if (e == 16 && vec) k_logprobs_part<16, true><<<grid, LP_THREADS, lp_smem(16), st>>>(a);
+  else if (e == 16) k_logprobs_part<16, false><<<grid, LP_THREADS, 0, st>>>(a);
+  else if (vec) k_logprobs_part<32, true><<<grid, LP_THREADS, lp_smem(32), st>>>(a);
+  else k_logprobs_part<32, false><<<grid, LP_THREADS, 0, st>>>(a);
+  CUDA_TRY(cudaGetLastError());
+  if (a.slices > 1) {  // launched early: it waits for the slices itself
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(n);
+    cfg.blockDim = dim3(LP_JOIN);
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    CUDA_TRY(cudaLaunchKernelEx(&cfg, k_logprobs_join, a));
   }
+  return L3G_OK;
+}
+
+// Synchronizes the device; the error word of the kernels' bounded waits.
+extern "C" int l3g_logprobs_status(l3g_logprobs* h, int32_t* err, int32_t* where) {
+  if (!h || !err || !where) return l3g_fail(L3G_E_INVALID, "null argument");
+  ON_DEVICE(h->device);
+  CUDA_TRY(cudaDeviceSynchronize());
+  Result r{};
+  CUDA_TRY(cudaMemcpy(&r, h->d_res, sizeof r, cudaMemcpyDeviceToHost));
+  CUDA_TRY(cudaMemset(h->d_res, 0, sizeof(Result)));
+  *err = r.err;
+  *where = r.where;
   return L3G_OK;
 }
 

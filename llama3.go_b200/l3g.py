@@ -165,6 +165,7 @@ def lib():
         "l3g_logprobs_free": (None, [_P]),
         "l3g_logprobs_run": (C.c_int, [_P, _P, C.c_int64, C.c_int32, _P, _P, _P, _P, C.c_int32, _P, _P,
                                        _P]),
+        "l3g_logprobs_status": (C.c_int, [_P, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
         "l3g_kv_copy_pages": (C.c_int, [_P, C.c_int32, _P, C.c_int32, C.c_int32, _P, _P, _P, C.c_int32,
                                         _P, _P]),
         "l3g_state_read_kv": (C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32,
@@ -834,6 +835,12 @@ class LogProbs:
         _check(lib().l3g_logprobs_run(self._h, logits_ptr or None, ld, n, targets_ptr or None,
                                       logprob_ptr or None, entropy_ptr or None, rank_ptr or None, top_k,
                                       top_ids_ptr or None, top_logprobs_ptr or None, stream or None))
+
+    def status(self):
+        """(err, where) of the calls since the last status()."""
+        e, w = C.c_int32(), C.c_int32()
+        _check(lib().l3g_logprobs_status(self._h, C.byref(e), C.byref(w)))
+        return e.value, w.value
 
     def Close(self):
         if self._h:
