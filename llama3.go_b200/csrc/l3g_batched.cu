@@ -361,6 +361,15 @@ static cudaError_t launch_pf_attention(const l3g_model* m, const l3g_workspace* 
   return cudaGetLastError();
 }
 
+// Zero the activation chunks of n_tok tokens where columns pad them: the layout
+// depends on the number of tokens and columns, so another call's bytes lie
+// there, and a scale that is NaN spoils a product with zero weights.
+static cudaError_t clear_padding(uint8_t* act, int n_tok, int nt, int cols, cudaStream_t st) {
+  if (cols % (gemm::BPC * 32) == 0) return cudaSuccess;
+  const size_t tiles = (size_t)(n_tok + nt - 1) / nt;
+  return cudaMemsetAsync(act, 0, tiles * gemm::chunks(cols) * gemm::b_chunk(nt), st);
+}
+
 // One pass of P <= pf_cap tokens at positions pos0..pos0+P-1 over every
 // layer.  The last layer stops after its K/V append: its attention and FFN
 // outputs only feed the logits, which prefill does not compute (infer.go:250).
@@ -380,6 +389,7 @@ static int enqueue_prefill_pass(l3g_model* m, l3g_state* s, l3g_workspace* ws, i
     const LayerW& L = m->layers[l];
     const KvMap kv = state_kv(s);
     // residual (from layer l-1's down) -> RMSNorm -> act-quant, infer.go:67-73
+    CUDA_TRY(clear_padding(act, P, nt, ne, st));
     k_pf_rms_quant<<<P, PF_THREADS, 0, st>>>(ws->pf_x, l ? ws->pf_y : nullptr, L.attn_norm,
                                             hp.rms_eps, ne, nt, gemm::chunks(ne), act);
     CUDA_TRY(cudaGetLastError());
@@ -414,12 +424,14 @@ static int enqueue_prefill_pass(l3g_model* m, l3g_state* s, l3g_workspace* ws, i
                                  st));
     // residual -> RMSNorm -> act-quant -> up/gate -> SwiGLU -> act-quant,
     // infer.go:189-234
+    CUDA_TRY(clear_padding(act, P, nt, ne, st));
     k_pf_rms_quant<<<P, PF_THREADS, 0, st>>>(ws->pf_x, ws->pf_y, L.ffn_norm, hp.rms_eps, ne, nt,
                                             gemm::chunks(ne), act);
     CUDA_TRY(cudaGetLastError());
     CUDA_TRY(launch_gemm(L.gupgate, act, P, ws->pf_ug, ws->d_res, wait_ns, m->nsm, st, 0,
                          ws->pf_part, ws->pf_part_floats));
     {
+      CUDA_TRY(clear_padding(act, P, nt, m->ff_l, st));
       const long long warps = (long long)P * (m->ff_l / 32);
       k_pf_swiglu_quant<<<(unsigned)((warps * 32 + 255) / 256), 256, 0, st>>>(
           ws->pf_ug, P, m->ff_l, nt, gemm::chunks(m->ff_l), act);
@@ -665,6 +677,7 @@ extern "C" int l3g_batch_step(l3g_batch* b, l3g_state* const* states, int32_t n,
   CUDA_TRY(cudaGetLastError());
   for (int l = 0; l < hp.n_layers; ++l) {
     const LayerW& L = m->layers[l];
+    CUDA_TRY(clear_padding(b->act, n, nt, ne, st));
     k_pf_rms_quant<<<n, PF_THREADS, 0, st>>>(b->x, l ? b->y : nullptr, L.attn_norm, hp.rms_eps,
                                             ne, nt, gemm::chunks(ne), b->act);
     CUDA_TRY(cudaGetLastError());
@@ -722,12 +735,14 @@ extern "C" int l3g_batch_step(l3g_batch* b, l3g_state* const* states, int32_t n,
                          b->part_floats));
     if (m->world > 1)
       NCCL_TRY(nccl()->AllReduce(b->y, b->y, (size_t)n * ne, ncclFloat, ncclSum, m->comm, st));
+    CUDA_TRY(clear_padding(b->act, n, nt, ne, st));
     k_pf_rms_quant<<<n, PF_THREADS, 0, st>>>(b->x, b->y, L.ffn_norm, hp.rms_eps, ne, nt,
                                             gemm::chunks(ne), b->act);
     CUDA_TRY(cudaGetLastError());
     CUDA_TRY(launch_gemm(L.gupgate, b->act, n, b->ug, b->d_res, wait_ns, m->nsm, st, 0, b->part,
                          b->part_floats));
     {
+      CUDA_TRY(clear_padding(b->act, n, nt, m->ff_l, st));
       const long long warps = (long long)n * (m->ff_l / 32);
       k_pf_swiglu_quant<<<(unsigned)((warps * 32 + 255) / 256), 256, 0, st>>>(
           b->ug, n, m->ff_l, nt, gemm::chunks(m->ff_l), b->act);
@@ -739,6 +754,7 @@ extern "C" int l3g_batch_step(l3g_batch* b, l3g_state* const* states, int32_t n,
       NCCL_TRY(nccl()->AllReduce(b->y, b->y, (size_t)n * ne, ncclFloat, ncclSum, m->comm, st));
   }
   // residual -> final RMSNorm -> act-quant -> logits shard, infer.go:250-260
+  CUDA_TRY(clear_padding(b->act, n, nt, ne, st));
   k_pf_rms_quant<<<n, PF_THREADS, 0, st>>>(b->x, b->y, m->out_norm, hp.rms_eps, ne, nt,
                                           gemm::chunks(ne), b->act);
   CUDA_TRY(cudaGetLastError());
