@@ -174,6 +174,22 @@ int l3g_kvpool_free_pages(l3g_kvpool *p, int32_t *n);
 int l3g_state_new_in_pool(l3g_model *m, l3g_kvpool *pool, int32_t ctx_len,
                           l3g_state **out);
 int l3g_state_pages(const l3g_state *s, int32_t *mapped);
+/* A new state that holds src's positions [0, n_pos) (n_pos < 0: its own
+ * position) and continues from there; ctx_len <= 0 means src's.  In a shared
+ * pool the two share the pages: nothing is copied until one of them writes to
+ * a page that the other maps too, which then gives the writer a copy of its
+ * own (a step that finds no free page for it fails with L3G_E_CTX).  A state
+ * with a private pool is copied. */
+int l3g_state_fork(const l3g_state *src, int32_t n_pos, int32_t ctx_len,
+                   l3g_state **out);
+/* Gives the pages behind the state's position back to its shared pool (after
+ * l3g_state_set_pos moved it back): positions from there on are forgotten. */
+int l3g_state_trim(l3g_state *s);
+/* Moves the pages in use to the lowest ids, in the order of the states: then
+ * the pages of a state's (layer, kv head) follow one another, and a snapshot
+ * or a restore needs one copy for each.  No step of the pool's states may run.
+ * *moved receives the pages that moved. */
+int l3g_kvpool_compact(l3g_kvpool *p, int32_t *moved);
 int l3g_state_pos(const l3g_state *s, int32_t *pos);
 int l3g_state_ctx_len(const l3g_state *s, int32_t *ctx_len);
 /* Moves the write position (0 <= pos <= ctx): rewinds a session for reuse
@@ -433,6 +449,29 @@ int l3g_batch_step(l3g_batch *b, l3g_state *const *states, int32_t n,
                    const int32_t *tokens, int32_t top_k, float temperature,
                    const uint64_t *seeds, int32_t *next_tokens,
                    float *logits_out);
+/* Extends n sessions by chunks of given tokens: state i ingests the next
+ * n_tokens[i] of `tokens` (the sessions' chunks one after another, T in all;
+ * a chunk may be empty) at its position and advances by as many.  A pass of up
+ * to 512 tokens of any sessions runs the products of l3g_batch_step over all of
+ * them and their attention as one l3g_chunk_attn call.  With score != NULL the
+ * logits after each token are computed and described (l3g_logprobs_run): for
+ * token i of T the log probability and rank of targets[i] (nullable), usually
+ * the token that follows, the entropy, and the top_k alternatives.  score's
+ * arrays are HOST arrays of T entries ([T][top_k] the last two), each nullable.
+ * One GPU (no tensor parallelism).  On failure the states' positions are those
+ * of the last completed pass.  (The reference ingests one session's tokens one
+ * by one and keeps the last token's logits, main.go:276-286.) */
+typedef struct {
+  float *logprob;
+  float *entropy;
+  int32_t *rank;
+  int32_t top_k;
+  int32_t *top_ids;
+  float *top_logprobs;
+} l3g_score;
+int l3g_batch_extend(l3g_batch *b, l3g_state *const *states, int32_t n,
+                     const int32_t *n_tokens, const int32_t *tokens,
+                     const int32_t *targets, const l3g_score *score);
 
 /* ---- batched Q8_0 product on the tensor cores (tcgen05 kind::i8) --------- */
 /* n_tok independent Q8_0 matvecs over one weight matrix, as one GEMM:

@@ -468,7 +468,7 @@ extern "C" int l3g_prefill_batched(l3g_model* m, l3g_state* s, l3g_workspace* ws
   if (int rc = gemm_setup()) return rc;
   if (int rc = ensure_gemm_weights(m)) return rc;
   if (int rc = ensure_prefill_buffers(ws)) return rc;
-  if (int rc = state_map(s, s->pos + n, ws->stream)) return rc;
+  if (int rc = state_map(s, s->pos, s->pos + n, ws->stream)) return rc;
   ws->logits_valid = false;
   for (int c0 = 0; c0 < n; c0 += ws->pf_cap) {
     const int P = std::min(ws->pf_cap, n - c0);
@@ -492,7 +492,44 @@ extern "C" int l3g_prefill_batched(l3g_model* m, l3g_state* s, l3g_workspace* ws
 // ---------------------------------------------------------------------------
 // batched decode
 // ---------------------------------------------------------------------------
+// Tokens of any sessions per pass of l3g_batch_extend, and rows of logits that
+// are held at once.
+constexpr int EXT_CAP = 512, EXT_LOGITS = 128;
+// Its buffers, made by the first call.
+struct ExtBuf {
+  l3g_chunk_attn* attn = nullptr;
+  l3g_logprobs* lp = nullptr;
+  SeqInfo* h_rows = nullptr;        // pinned [EXT_CAP]: a pass's tokens
+  SeqInfo* d_rows = nullptr;
+  l3g_chunk_seq* h_seqs = nullptr;  // pinned [cap]: its sessions
+  l3g_chunk_seq* d_seqs = nullptr;
+  int* h_targets = nullptr;         // pinned [EXT_CAP]
+  int* d_targets = nullptr;
+  Result* h_res = nullptr;          // pinned [3]: the error words
+  float *x = nullptr, *y = nullptr, *qkv = nullptr, *q = nullptr, *att = nullptr, *ug = nullptr;
+  uint8_t* act = nullptr;
+  float* part = nullptr;            // split-K partial sums of the product
+  size_t part_floats = 0;
+  float* logits = nullptr;          // [EXT_LOGITS][v_l]
+  float *logprob = nullptr, *entropy = nullptr, *top_lp = nullptr;  // [EXT_CAP] ([MAX_TOPK])
+  int *rank = nullptr, *top_ids = nullptr;
+};
+static void ext_free(ExtBuf* e) {
+  if (!e) return;
+  l3g_chunk_attn_free(e->attn);
+  l3g_logprobs_free(e->lp);
+  void* d[] = {e->d_rows, e->d_seqs, e->d_targets, e->x, e->y, e->qkv, e->q, e->att, e->ug, e->act,
+               e->part, e->logits, e->logprob, e->entropy, e->top_lp, e->rank, e->top_ids};
+  for (void* p : d)
+    if (p) cudaFree(p);
+  void* h[] = {e->h_rows, e->h_seqs, e->h_targets, e->h_res};
+  for (void* p : h)
+    if (p) cudaFreeHost(p);
+  delete e;
+}
+
 struct l3g_batch {
+  ExtBuf* ext = nullptr;
   l3g_model* m = nullptr;
   int device = 0, cap = 0, max_splits = 0, tk_chunks = 0;
   cudaStream_t stream = nullptr;
@@ -531,6 +568,7 @@ extern "C" void l3g_batch_free(l3g_batch* b) {
   void* h[] = {b->h_seq, b->h_out, b->h_res};
   for (void* p : h)
     if (p) cudaFreeHost(p);
+  ext_free(b->ext);
   if (b->stream) cudaStreamDestroy(b->stream);
   delete b;
 }
@@ -669,7 +707,7 @@ extern "C" int l3g_batch_step(l3g_batch* b, l3g_state* const* states, int32_t n,
   const int splits = (max_pos + 1 + split_len - 1) / split_len;
   const float scale = (float)(1.0 / sqrt((double)hd));
   for (int i = 0; i < n; ++i)  // each session's page for this step's position
-    if (int rc = state_map(states[i], states[i]->pos + 1, st)) return rc;
+    if (int rc = state_map(states[i], states[i]->pos, states[i]->pos + 1, st)) return rc;
   CUDA_TRY(cudaMemcpyAsync(b->d_seq, b->h_seq, (size_t)n * sizeof(SeqInfo),
                            cudaMemcpyHostToDevice, st));
   k_bd_embed<<<dim3((ne + 255) / 256, n), 256, 0, st>>>(m->emb, hp.vocab_size, ne, b->d_seq, b->x,
@@ -802,6 +840,251 @@ extern "C" int l3g_batch_step(l3g_batch* b, l3g_state* const* states, int32_t n,
   for (int i = 0; i < n; ++i) {
     next_tokens[i] = b->h_out[i].token;
     states[i]->pos++;
+  }
+  return L3G_OK;
+}
+
+// ---------------------------------------------------------------------------
+// chunks of tokens for many sessions
+// ---------------------------------------------------------------------------
+static int ensure_ext(l3g_batch* b) {
+  if (b->ext) return L3G_OK;
+  const l3g_model* m = b->m;
+  const int ne = m->hp.n_emb, nq = m->hq_l * m->hd, nkv = m->hkv_l * m->hd;
+  uint64_t act_bytes = 0;
+  if (int rc = l3g_gemm_act_bytes(EXT_CAP, std::max(std::max(ne, nq), m->ff_l), &act_bytes))
+    return rc;
+  auto* x = new ExtBuf();
+  int rc = l3g_chunk_attn_new(m->hq_l, m->hkv_l, m->hd, m->kv_f16 ? L3G_KV_F16 : L3G_KV_F32,
+                              m->device, &x->attn);
+  if (!rc) rc = l3g_logprobs_new(EXT_LOGITS, m->hp.vocab_size, m->device, &x->lp);
+  if (rc) {
+    ext_free(x);
+    return rc;
+  }
+  const size_t cap = EXT_CAP;
+  x->part_floats = gemm_part_bound(m->glogits, EXT_LOGITS, m->nsm);
+  for (const auto& L : m->layers)
+    for (const GemmMat* g : {&L.gqkv, &L.gwo, &L.gupgate, &L.gdown})
+      x->part_floats = std::max(x->part_floats, gemm_part_bound(*g, EXT_CAP, m->nsm));
+  cudaError_t e = cudaMallocHost(&x->h_rows, cap * sizeof(SeqInfo));
+  if (e == cudaSuccess) e = cudaMallocHost(&x->h_seqs, (size_t)b->cap * sizeof(l3g_chunk_seq));
+  if (e == cudaSuccess) e = cudaMallocHost(&x->h_targets, cap * 4);
+  if (e == cudaSuccess) e = cudaMallocHost(&x->h_res, 3 * sizeof(Result));
+  if (e == cudaSuccess) e = cudaMalloc(&x->d_rows, cap * sizeof(SeqInfo));
+  if (e == cudaSuccess) e = cudaMalloc(&x->d_seqs, (size_t)b->cap * sizeof(l3g_chunk_seq));
+  if (e == cudaSuccess) e = cudaMalloc(&x->d_targets, cap * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&x->x, cap * ne * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&x->y, cap * ne * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&x->qkv, cap * (nq + 2 * nkv) * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&x->q, cap * nq * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&x->att, cap * nq * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&x->ug, cap * 2 * m->ff_l * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&x->act, act_bytes);
+  // padding tokens and columns of the activation chunks
+  if (e == cudaSuccess) e = cudaMemset(x->act, 0, act_bytes);
+  if (e == cudaSuccess && x->part_floats) e = cudaMalloc(&x->part, x->part_floats * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&x->logits, (size_t)EXT_LOGITS * m->v_l * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&x->logprob, cap * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&x->entropy, cap * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&x->rank, cap * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&x->top_ids, cap * MAX_TOPK * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&x->top_lp, cap * MAX_TOPK * 4);
+  if (e != cudaSuccess) {
+    ext_free(x);
+    return l3g_fail(L3G_E_CUDA, "batch extension buffers: %s", cudaGetErrorString(e));
+  }
+  b->ext = x;
+  return L3G_OK;
+}
+
+// One pass over P tokens (x->h_rows) of n_seqs sessions (x->h_seqs): every
+// layer, and with score the logits of each token, EXT_LOGITS rows at a time.
+static int enqueue_ext_pass(l3g_batch* b, int P, int n_seqs, bool targets, const l3g_score* score) {
+  l3g_model* m = b->m;
+  ExtBuf* x = b->ext;
+  const l3g_hparams& hp = m->hp;
+  const cudaStream_t st = b->stream;
+  const int ne = hp.n_emb, hd = m->hd, nq = m->hq_l * hd, nkv = m->hkv_l * hd;
+  const unsigned long long wait_ns = WAIT_TIMEOUT_NS;
+  const int nt = gemm::token_tile(P), n_pad = (P + nt - 1) / nt * nt;
+  CUDA_TRY(cudaMemcpyAsync(x->d_rows, x->h_rows, (size_t)P * sizeof(SeqInfo),
+                           cudaMemcpyHostToDevice, st));
+  CUDA_TRY(cudaMemcpyAsync(x->d_seqs, x->h_seqs, (size_t)n_seqs * sizeof(l3g_chunk_seq),
+                           cudaMemcpyHostToDevice, st));
+  k_bd_embed<<<dim3((ne + 255) / 256, P), 256, 0, st>>>(m->emb, hp.vocab_size, ne, x->d_rows, x->x,
+                                                        b->d_res);
+  CUDA_TRY(cudaGetLastError());
+  for (int l = 0; l < hp.n_layers; ++l) {
+    const LayerW& L = m->layers[l];
+    CUDA_TRY(clear_padding(x->act, P, nt, ne, st));
+    k_pf_rms_quant<<<P, PF_THREADS, 0, st>>>(x->x, l ? x->y : nullptr, L.attn_norm, hp.rms_eps, ne,
+                                            nt, gemm::chunks(ne), x->act);
+    CUDA_TRY(cudaGetLastError());
+    CUDA_TRY(launch_gemm(L.gqkv, x->act, P, x->qkv, b->d_res, wait_ns, m->nsm, st, 0, x->part,
+                         x->part_floats));
+    const long long pairs = (long long)P * ((nq + 2 * nkv) / 2);
+    k_bd_qkv_rope<<<(unsigned)((pairs + 255) / 256), 256, 0, st>>>(
+        x->qkv, P, x->d_rows, l, nq, nkv, hd, m->rope_half, x->q, m->kv_f16);
+    CUDA_TRY(cudaGetLastError());
+    // the last layer's attention and FFN feed only the logits
+    if (l == hp.n_layers - 1 && !score) break;
+    if (int rc = l3g_chunk_attn_run(x->attn, x->d_seqs, n_seqs, P, x->q, nq, x->att, nq, l, 0.0f,
+                                    st))
+      return rc;
+    const long long warps = (long long)n_pad * gemm::chunks(nq) * gemm::BPC;
+    k_gemm_quantize<<<(unsigned)((warps * 32 + 255) / 256), 256, 0, st>>>(
+        x->att, P, nq, nt, gemm::chunks(nq), n_pad, x->act);
+    CUDA_TRY(cudaGetLastError());
+    CUDA_TRY(launch_gemm(L.gwo, x->act, P, x->y, b->d_res, wait_ns, m->nsm, st, 0, x->part,
+                         x->part_floats));
+    CUDA_TRY(clear_padding(x->act, P, nt, ne, st));
+    k_pf_rms_quant<<<P, PF_THREADS, 0, st>>>(x->x, x->y, L.ffn_norm, hp.rms_eps, ne, nt,
+                                            gemm::chunks(ne), x->act);
+    CUDA_TRY(cudaGetLastError());
+    CUDA_TRY(launch_gemm(L.gupgate, x->act, P, x->ug, b->d_res, wait_ns, m->nsm, st, 0, x->part,
+                         x->part_floats));
+    CUDA_TRY(clear_padding(x->act, P, nt, m->ff_l, st));
+    const long long fw = (long long)P * (m->ff_l / 32);
+    k_pf_swiglu_quant<<<(unsigned)((fw * 32 + 255) / 256), 256, 0, st>>>(
+        x->ug, P, m->ff_l, nt, gemm::chunks(m->ff_l), x->act);
+    CUDA_TRY(cudaGetLastError());
+    CUDA_TRY(launch_gemm(L.gdown, x->act, P, x->y, b->d_res, wait_ns, m->nsm, st, 0, x->part,
+                         x->part_floats));
+  }
+  if (!score) return L3G_OK;
+  CUDA_TRY(clear_padding(x->act, P, nt, ne, st));
+  k_pf_rms_quant<<<P, PF_THREADS, 0, st>>>(x->x, x->y, m->out_norm, hp.rms_eps, ne, nt,
+                                          gemm::chunks(ne), x->act);
+  CUDA_TRY(cudaGetLastError());
+  if (targets)
+    CUDA_TRY(cudaMemcpyAsync(x->d_targets, x->h_targets, (size_t)P * 4, cudaMemcpyHostToDevice, st));
+  for (int r0 = 0; r0 < P; r0 += EXT_LOGITS) {
+    const int rows = std::min(EXT_LOGITS, P - r0);
+    // the chunks of a pass of more than 64 tokens are laid out in tiles of 128
+    // (a token tile is EXT_LOGITS rows); a last tile of fewer is computed with
+    // as many of its padding tokens as keep that layout
+    const int n_tok = nt == 128 ? std::max(rows, 65) : rows;
+    const uint8_t* act = x->act + (size_t)(r0 / nt) * gemm::chunks(ne) * gemm::b_chunk(nt);
+    CUDA_TRY(launch_gemm(m->glogits, act, n_tok, x->logits, b->d_res, wait_ns, m->nsm, st, m->v_l,
+                         x->part, x->part_floats));
+    if (int rc = l3g_logprobs_run(
+            x->lp, x->logits, m->v_l, rows, targets ? x->d_targets + r0 : nullptr,
+            targets && score->logprob ? x->logprob + r0 : nullptr,
+            score->entropy ? x->entropy + r0 : nullptr,
+            targets && score->rank ? x->rank + r0 : nullptr, score->top_k,
+            score->top_ids ? x->top_ids + (size_t)r0 * score->top_k : nullptr,
+            score->top_logprobs ? x->top_lp + (size_t)r0 * score->top_k : nullptr, st))
+      return rc;
+  }
+  return L3G_OK;
+}
+
+extern "C" int l3g_batch_extend(l3g_batch* b, l3g_state* const* states, int32_t n,
+                                const int32_t* n_tokens, const int32_t* tokens,
+                                const int32_t* targets, const l3g_score* score) {
+  if (!b || !states || !n_tokens) return l3g_fail(L3G_E_INVALID, "null argument");
+  l3g_model* m = b->m;
+  if (m->world > 1) return l3g_fail(L3G_E_INVALID, "batch extension runs on one GPU");
+  if (n <= 0 || n > b->cap) return l3g_fail(L3G_E_INVALID, "n=%d outside [1, %d]", n, b->cap);
+  if (score) {
+    if (score->top_k < 0 || score->top_k > MAX_TOPK || score->top_k > m->hp.vocab_size)
+      return l3g_fail(L3G_E_INVALID, "top_k=%d outside [0, %d]", score->top_k,
+                      std::min(MAX_TOPK, m->hp.vocab_size));
+    if (!targets && (score->logprob || score->rank))
+      return l3g_fail(L3G_E_INVALID, "log probabilities and ranks need targets");
+  }
+  long long total = 0;
+  for (int i = 0; i < n; ++i) {
+    const l3g_state* s = states[i];
+    if (!s) return l3g_fail(L3G_E_INVALID, "null state %d", i);
+    if (s->m != m) return l3g_fail(L3G_E_INVALID, "state %d belongs to another model", i);
+    for (int j = 0; j < i; ++j)
+      if (states[j] == s) return l3g_fail(L3G_E_INVALID, "state %d appears twice", i);
+    if (n_tokens[i] < 0) return l3g_fail(L3G_E_INVALID, "n_tokens[%d]=%d", i, n_tokens[i]);
+    if ((long long)s->pos + n_tokens[i] > s->ctx)
+      return l3g_fail(L3G_E_CTX, "context length exceeded (%d)", s->ctx);
+    total += n_tokens[i];
+  }
+  if (total == 0) return L3G_OK;
+  if (total > INT_MAX) return l3g_fail(L3G_E_INVALID, "%lld tokens", total);
+  if (!tokens) return l3g_fail(L3G_E_INVALID, "null argument");
+  for (long long t = 0; t < total; ++t)
+    if (tokens[t] < 0 || tokens[t] >= m->hp.vocab_size)
+      return l3g_fail(L3G_E_TOKEN, "token out of range: %d", tokens[t]);
+  CUDA_TRY(cudaSetDevice(m->device));
+  if (int rc = ensure_ext(b)) return rc;
+  ExtBuf* x = b->ext;
+  const cudaStream_t st = b->stream;
+  for (int i = 0; i < n; ++i)  // each session's pages
+    if (n_tokens[i] > 0)
+      if (int rc = state_map(states[i], states[i]->pos, states[i]->pos + n_tokens[i], st)) return rc;
+  int seq = 0, seq_done = 0;  // the next token: session and place in its chunk
+  for (long long t0 = 0; t0 < total;) {
+    const int P = (int)std::min<long long>(EXT_CAP, total - t0);
+    int n_seqs = 0;
+    std::vector<std::pair<int, int>> took;
+    for (int row = 0; row < P;) {
+      while (seq_done == n_tokens[seq]) ++seq, seq_done = 0;
+      l3g_state* s = states[seq];
+      const int k = std::min(P - row, n_tokens[seq] - seq_done);
+      l3g_chunk_seq& d = x->h_seqs[n_seqs++];
+      d = l3g_chunk_seq{};
+      d.pool = s->pool->base;
+      d.pages = s->d_pages;
+      d.n_pages = s->pool->n_pages;
+      d.pps = s->pps;
+      d.q0 = row;
+      d.n_q = k;
+      d.kv_len = s->pos + k;
+      for (int i = 0; i < k; ++i) {
+        SeqInfo& q = x->h_rows[row + i];
+        q = SeqInfo{};
+        q.kv_pool = s->pool->base;
+        q.kv_pages = s->d_pages;
+        q.kv_pps = s->pps;
+        q.rope_cos = s->rope_cos;
+        q.rope_sin = s->rope_sin;
+        q.ctx = s->ctx;
+        q.pos = s->pos + i;
+        q.token = tokens[t0 + row + i];
+      }
+      took.push_back({seq, k});
+      seq_done += k;
+      row += k;
+    }
+    if (targets) std::copy(targets + t0, targets + t0 + P, x->h_targets);
+    int rc = enqueue_ext_pass(b, P, n_seqs, targets != nullptr, score);
+    cudaError_t e = cudaSuccess;
+    auto fetch = [&](void* dst, const void* src, size_t bytes) {
+      if (dst && bytes && e == cudaSuccess)
+        e = cudaMemcpyAsync(dst, src, bytes, cudaMemcpyDeviceToHost, st);
+    };
+    fetch(&x->h_res[0], b->d_res, sizeof(Result));
+    fetch(&x->h_res[1], chunk_attn_word(x->attn), sizeof(Result));
+    fetch(&x->h_res[2], logprobs_word(x->lp), sizeof(Result));
+    if (!rc && score) {
+      const size_t k = (size_t)score->top_k;
+      if (targets && score->logprob) fetch(score->logprob + t0, x->logprob, (size_t)P * 4);
+      if (targets && score->rank) fetch(score->rank + t0, x->rank, (size_t)P * 4);
+      if (score->entropy) fetch(score->entropy + t0, x->entropy, (size_t)P * 4);
+      if (score->top_ids) fetch(score->top_ids + t0 * k, x->top_ids, (size_t)P * k * 4);
+      if (score->top_logprobs) fetch(score->top_logprobs + t0 * k, x->top_lp, (size_t)P * k * 4);
+    }
+    const cudaError_t e2 = cudaStreamSynchronize(st);
+    if (rc) return rc;
+    CUDA_TRY(e);
+    CUDA_TRY(e2);
+    for (int w = 0; w < 3; ++w) {
+      if (!x->h_res[w].err) continue;
+      const int code = x->h_res[w].err, where = x->h_res[w].where;
+      Result* words[3] = {b->d_res, chunk_attn_word(x->attn), logprobs_word(x->lp)};
+      for (Result* r : words) cudaMemset(r, 0, sizeof(Result));
+      return l3g_fail(L3G_E_DEVICE, "device check failed: code %d at site %d (%s)", code, where,
+                      code == ERR_TIMEOUT ? "bounded wait ran out" : "bad input");
+    }
+    for (const auto& s : took) states[s.first]->pos += s.second;
+    t0 += P;
   }
   return L3G_OK;
 }

@@ -155,7 +155,9 @@ __device__ __forceinline__ bool chunk_wait(uint64_t* b, uint32_t parity, ChunkSm
 // Whether a descriptor stays inside its bounds (its pages are checked where
 // they are read).
 __device__ __forceinline__ bool chunk_seq_ok(const l3g_chunk_seq& s, int total_q) {
-  return s.pool && s.pages && s.pps >= 0 && s.q0 >= 0 && s.n_q >= 0 && s.n_q <= total_q &&
+  // (a tensor copy needs a 16-byte aligned base)
+  return s.pool && s.pages && ((uintptr_t)s.pool & 15) == 0 && ((uintptr_t)s.pages & 3) == 0 &&
+         s.pps >= 0 && s.q0 >= 0 && s.n_q >= 0 && s.n_q <= total_q &&
          s.q0 <= total_q - s.n_q && s.kv_len >= 0 &&
          (long long)s.kv_len <= (long long)s.pps * KV_PAGE;
 }

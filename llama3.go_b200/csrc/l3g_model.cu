@@ -2,6 +2,8 @@
 // snapshots.
 #include "l3g_rt.h"
 
+#include "l3g_pages_plan.h"
+
 // ---------------------------------------------------------------------------
 // tiled Q8_0 matrices
 // ---------------------------------------------------------------------------
@@ -465,6 +467,7 @@ static int pool_create(l3g_model* m, int n_pages, bool priv, l3g_kvpool** out) {
                     (unsigned long long)bytes, cudaGetErrorString(e));
   }
   if (!priv) {  // a stack: the lowest ids come out first
+    p->refs.assign(n_pages, 0);
     p->free_pages.resize(n_pages);
     for (int i = 0; i < n_pages; ++i) p->free_pages[i] = n_pages - 1 - i;
   }
@@ -477,19 +480,33 @@ static void pool_destroy(l3g_kvpool* p) {
   cudaGetDevice(&prev);
   cudaSetDevice(p->device);
   if (p->base) cudaFree(p->base);
+  if (p->d_ids) cudaFree(p->d_ids);
   cudaSetDevice(prev);
   delete p;
 }
 
-// A state leaves its pool: its pages go back on the free list; a released
-// (or private) pool without states is destroyed.
-static void pool_leave(l3g_kvpool* p, const std::vector<int>& pages) {
+// A state lets go of a page (the pool is locked): free once no state maps it.
+static void page_drop(l3g_kvpool* p, int id) {
+  if (--p->refs[id] == 0) p->free_pages.push_back(id);
+}
+static int page_take(l3g_kvpool* p) {
+  const int id = p->free_pages.back();
+  p->free_pages.pop_back();
+  p->refs[id] = 1;
+  return id;
+}
+
+// A state leaves its pool: the pages that no other state maps go back on the
+// free list; a released (or private) pool without states is destroyed.
+static void pool_leave(l3g_kvpool* p, l3g_state* s) {
   bool destroy = false;
   {
     std::lock_guard<std::mutex> lk(p->mu);
-    if (!p->priv)
-      for (int id : pages)
-        if (id >= 0) p->free_pages.push_back(id);
+    if (!p->priv) {
+      for (int id : s->h_pages)
+        if (id >= 0) page_drop(p, id);
+      p->members.erase(std::remove(p->members.begin(), p->members.end(), s), p->members.end());
+    }
     --p->states;
     destroy = p->priv || (p->released && p->states == 0);
   }
@@ -506,30 +523,81 @@ KvMap state_kv(const l3g_state* s) {
   return k;
 }
 
-int state_map(l3g_state* s, int n_pos, cudaStream_t st) {
+// Copies rows of pages, one list entry {source, destination, rows} each, from
+// src_pool to dst_pool on stream st and waits for them.  The lists go through
+// `ids` of `via` (locked by the caller).
+static int copy_pages(l3g_kvpool* via, const uint8_t* src_base, int n_src, uint8_t* dst_base,
+                      int n_dst, size_t page_bytes, const std::vector<int>& src,
+                      const std::vector<int>& dst, const std::vector<int>& rows, cudaStream_t st) {
+  const int n = (int)src.size();
+  if (n == 0) return L3G_OK;
+  if (via->ids_cap < 3 * n) {
+    if (via->d_ids) cudaFree(via->d_ids);
+    via->d_ids = nullptr;
+    via->ids_cap = 0;
+    CUDA_TRY(cudaMalloc(&via->d_ids, (size_t)3 * n * sizeof(int)));
+    via->ids_cap = 3 * n;
+  }
+  std::vector<int> all(src);
+  all.insert(all.end(), dst.begin(), dst.end());
+  all.insert(all.end(), rows.begin(), rows.end());
+  CUDA_TRY(cudaMemcpyAsync(via->d_ids, all.data(), all.size() * sizeof(int),
+                           cudaMemcpyHostToDevice, st));
+  if (int rc = l3g_kv_copy_pages(src_base, n_src, dst_base, n_dst, (int)(page_bytes / KV_PAGE),
+                                 via->d_ids, via->d_ids + n, via->d_ids + 2 * n, n, nullptr, st))
+    return rc;
+  CUDA_TRY(cudaStreamSynchronize(st));
+  return L3G_OK;
+}
+
+int state_map(l3g_state* s, int pos0, int n_pos, cudaStream_t st) {
   const int need = std::min(s->pps, (n_pos + KV_PAGE - 1) / KV_PAGE);
-  if (need <= s->mapped) return L3G_OK;
   const int heads = s->m->hp.n_layers * s->m->hkv_l;
   l3g_kvpool* p = s->pool;
-  {
+  int first = s->mapped, last = need;  // the table columns that change
+  if (!p->priv) {
     std::lock_guard<std::mutex> lk(p->mu);
-    const size_t want = (size_t)heads * (need - s->mapped);
+    // pages of the range that other states map too
+    std::vector<size_t> shared;
+    for (int j = pos0 / KV_PAGE; j < std::min(need, s->mapped); ++j)
+      for (int h = 0; h < heads; ++h)
+        if (p->refs[s->h_pages[(size_t)h * s->pps + j]] > 1) shared.push_back((size_t)h * s->pps + j);
+    const size_t want = shared.size() + (size_t)heads * std::max(0, need - s->mapped);
     if (p->free_pages.size() < want)
       return l3g_fail(L3G_E_CTX, "KV pool exhausted: %zu free pages, %zu needed for position %d",
                       p->free_pages.size(), want, n_pos - 1);
-    for (int j = s->mapped; j < need; ++j)
-      for (int h = 0; h < heads; ++h) {
-        s->h_pages[(size_t)h * s->pps + j] = p->free_pages.back();
-        p->free_pages.pop_back();
+    if (!shared.empty()) {
+      std::vector<int> src, dst, rows;
+      for (size_t e : shared) {
+        src.push_back(s->h_pages[e]);
+        dst.push_back(page_take(p));
+        const int j = (int)(e % s->pps);
+        rows.push_back(std::max(0, std::min(KV_PAGE, s->high - j * KV_PAGE)));
       }
+      if (int rc = copy_pages(p, p->base, p->n_pages, p->base, p->n_pages, p->page_bytes, src, dst,
+                              rows, st)) {
+        for (int id : dst) page_drop(p, id);
+        return rc;
+      }
+      for (size_t i = 0; i < shared.size(); ++i) {
+        page_drop(p, src[i]);
+        s->h_pages[shared[i]] = dst[i];
+        first = std::min(first, (int)(shared[i] % s->pps));
+      }
+      last = std::max(last, std::min(need, s->mapped));
+    }
+    for (int j = s->mapped; j < need; ++j)
+      for (int h = 0; h < heads; ++h) s->h_pages[(size_t)h * s->pps + j] = page_take(p);
   }
+  s->high = std::max(s->high, n_pos);
+  if (first >= last) return L3G_OK;
   // the new entries of every (layer, kv head): one 2-D copy (pageable
   // source: staged before the call returns)
-  CUDA_TRY(cudaMemcpy2DAsync(s->d_pages + s->mapped, (size_t)s->pps * sizeof(int),
-                             s->h_pages.data() + s->mapped, (size_t)s->pps * sizeof(int),
-                             (size_t)(need - s->mapped) * sizeof(int), (size_t)heads,
+  CUDA_TRY(cudaMemcpy2DAsync(s->d_pages + first, (size_t)s->pps * sizeof(int),
+                             s->h_pages.data() + first, (size_t)s->pps * sizeof(int),
+                             (size_t)(last - first) * sizeof(int), (size_t)heads,
                              cudaMemcpyHostToDevice, st));
-  s->mapped = need;
+  s->mapped = std::max(s->mapped, need);
   return L3G_OK;
 }
 
@@ -569,7 +637,7 @@ extern "C" void l3g_state_free(l3g_state* s) {
   if (s->d_pages) cudaFree(s->d_pages);
   if (s->rope_cos) cudaFree(s->rope_cos);
   if (s->rope_sin) cudaFree(s->rope_sin);
-  if (s->pool) pool_leave(s->pool, s->h_pages);
+  if (s->pool) pool_leave(s->pool, s);
   delete s;
 }
 
@@ -603,6 +671,7 @@ static int state_create(l3g_model* m, l3g_kvpool* pool, int32_t ctx, l3g_state**
         return l3g_fail(L3G_E_INVALID, "KV pool already freed");
       }
       ++pool->states;
+      pool->members.push_back(s);
     }
     s->pool = pool;
     // unmapped entries point at page 0 until mapped: never read, since a
@@ -653,6 +722,146 @@ extern "C" int l3g_state_new_in_pool(l3g_model* m, l3g_kvpool* pool, int32_t ctx
                                      l3g_state** out) {
   if (!pool) return l3g_fail(L3G_E_INVALID, "null argument");
   return state_create(m, pool, ctx, out);
+}
+
+extern "C" int l3g_state_fork(const l3g_state* src, int32_t n_pos, int32_t ctx,
+                              l3g_state** out) {
+  if (!src || !out) return l3g_fail(L3G_E_INVALID, "null argument");
+  *out = nullptr;
+  if (n_pos < 0) n_pos = src->pos;
+  if (n_pos > src->high)
+    return l3g_fail(L3G_E_INVALID, "fork at position %d of a state written up to %d", n_pos,
+                    src->high);
+  if (ctx <= 0) ctx = src->ctx;
+  ctx = std::min(ctx, src->m->hp.ctx_len);
+  if (n_pos > ctx) return l3g_fail(L3G_E_CTX, "context length exceeded (%d)", ctx);
+  l3g_kvpool* p = src->pool;
+  l3g_state* s = nullptr;
+  if (int rc = state_create(src->m, p->priv ? nullptr : p, ctx, &s)) return rc;
+  const int heads = s->m->hp.n_layers * s->m->hkv_l;
+  const int pages = (n_pos + KV_PAGE - 1) / KV_PAGE;
+  cudaError_t e = cudaSuccess;
+  int rc = L3G_OK;
+  if (p->priv) {  // its own pool: the rows are copied
+    std::vector<int> from, to, rows;
+    for (int h = 0; h < heads; ++h)
+      for (int j = 0; j < pages; ++j) {
+        from.push_back(src->h_pages[(size_t)h * src->pps + j]);
+        to.push_back(s->h_pages[(size_t)h * s->pps + j]);
+        rows.push_back(std::min(KV_PAGE, n_pos - j * KV_PAGE));
+      }
+    e = cudaDeviceSynchronize();  // steps in flight on any stream
+    if (e == cudaSuccess)
+      rc = copy_pages(s->pool, p->base, p->n_pages, s->pool->base, s->pool->n_pages, p->page_bytes,
+                      from, to, rows, nullptr);
+  } else {  // the pages are shared until one of the states writes to them
+    {
+      std::lock_guard<std::mutex> lk(p->mu);
+      for (int h = 0; h < heads; ++h)
+        for (int j = 0; j < pages; ++j) {
+          const int id = src->h_pages[(size_t)h * src->pps + j];
+          s->h_pages[(size_t)h * s->pps + j] = id;
+          ++p->refs[id];
+        }
+    }
+    std::vector<int> table(s->h_pages);
+    for (int& id : table) id = std::max(id, 0);
+    e = cudaMemcpy(s->d_pages, table.data(), table.size() * sizeof(int), cudaMemcpyHostToDevice);
+    s->mapped = pages;
+  }
+  if (e != cudaSuccess) rc = l3g_fail(L3G_E_CUDA, "state fork: %s", cudaGetErrorString(e));
+  if (rc) {
+    l3g_state_free(s);
+    return rc;
+  }
+  s->pos = s->high = n_pos;
+  *out = s;
+  return L3G_OK;
+}
+
+extern "C" int l3g_state_trim(l3g_state* s) {
+  if (!s) return l3g_fail(L3G_E_INVALID, "null argument");
+  s->high = std::min(s->high, s->pos);
+  l3g_kvpool* p = s->pool;
+  const int keep = (s->pos + KV_PAGE - 1) / KV_PAGE;
+  if (p->priv || keep >= s->mapped) return L3G_OK;
+  const int heads = s->m->hp.n_layers * s->m->hkv_l;
+  std::lock_guard<std::mutex> lk(p->mu);
+  for (int h = 0; h < heads; ++h)
+    for (int j = keep; j < s->mapped; ++j) {
+      int& id = s->h_pages[(size_t)h * s->pps + j];
+      page_drop(p, id);
+      id = -1;
+    }
+  s->mapped = keep;  // (the device table's entries behind it are not read)
+  return L3G_OK;
+}
+
+extern "C" int l3g_kvpool_compact(l3g_kvpool* p, int32_t* moved) {
+  if (!p || !moved) return l3g_fail(L3G_E_INVALID, "null argument");
+  *moved = 0;
+  std::lock_guard<std::mutex> lk(p->mu);
+  // the pages in the order of states, (layer, kv head) and position; a page
+  // that several states map where the first of them has it
+  std::vector<int> order, place(p->n_pages, -1);
+  for (l3g_state* s : p->members) {
+    const int heads = s->m->hp.n_layers * s->m->hkv_l;
+    for (int h = 0; h < heads; ++h)
+      for (int j = 0; j < s->mapped; ++j) {
+        const int id = s->h_pages[(size_t)h * s->pps + j];
+        if (place[id] < 0) {
+          place[id] = (int)order.size();
+          order.push_back(id);
+        }
+      }
+  }
+  for (size_t t = 0; t < order.size(); ++t) *moved += order[t] != (int)t;
+  if (*moved == 0) return L3G_OK;
+  int prev = 0;
+  CUDA_TRY(cudaGetDevice(&prev));
+  CUDA_TRY(cudaSetDevice(p->device));
+  const int batch = (int)std::max<size_t>(1, std::min<size_t>(order.size(), (64u << 20) / p->page_bytes));
+  uint8_t* scratch = nullptr;
+  cudaError_t e = cudaMalloc(&scratch, (size_t)batch * p->page_bytes);
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();  // steps in flight on any stream
+  int rc = e == cudaSuccess ? L3G_OK
+                            : l3g_fail(L3G_E_CUDA, "KV pool compaction: %s", cudaGetErrorString(e));
+  if (!rc) {
+    auto copy = [&](const std::vector<std::pair<int, int>>& c, const uint8_t* from, int n_from,
+                    uint8_t* to, int n_to) {
+      std::vector<int> a, b, rows(c.size(), KV_PAGE);
+      for (const auto& x : c) {
+        a.push_back(x.first);
+        b.push_back(x.second);
+      }
+      return copy_pages(p, from, n_from, to, n_to, p->page_bytes, a, b, rows, nullptr);
+    };
+    // (a CUDA error between the rounds leaves the pool unusable, as any does)
+    for (const CompactRound& r : compact_plan(order, p->n_pages, batch)) {
+      if ((rc = copy(r.out, p->base, p->n_pages, scratch, batch))) break;
+      if ((rc = copy(r.away, p->base, p->n_pages, p->base, p->n_pages))) break;
+      if ((rc = copy(r.in, scratch, batch, p->base, p->n_pages))) break;
+    }
+  }
+  if (!rc) {
+    std::vector<int> refs(p->n_pages, 0);
+    for (size_t t = 0; t < order.size(); ++t) refs[t] = p->refs[order[t]];
+    p->refs.swap(refs);
+    p->free_pages.clear();
+    for (int id = p->n_pages - 1; id >= (int)order.size(); --id) p->free_pages.push_back(id);
+    for (l3g_state* s : p->members) {
+      std::vector<int> table(s->h_pages.size(), 0);
+      for (size_t i = 0; i < table.size(); ++i)
+        if (s->h_pages[i] >= 0) table[i] = s->h_pages[i] = place[s->h_pages[i]];
+      if (e == cudaSuccess)
+        e = cudaMemcpy(s->d_pages, table.data(), table.size() * sizeof(int), cudaMemcpyHostToDevice);
+    }
+    if (e != cudaSuccess)
+      rc = l3g_fail(L3G_E_CUDA, "KV pool compaction: %s", cudaGetErrorString(e));
+  }
+  if (scratch) cudaFree(scratch);
+  cudaSetDevice(prev);
+  return rc;
 }
 
 extern "C" int l3g_state_pages(const l3g_state* s, int32_t* mapped) {
@@ -778,7 +987,7 @@ extern "C" int l3g_state_restore(l3g_state* s, const void* src, uint64_t bytes) 
   if (bytes < snap_bytes(h)) return l3g_fail(L3G_E_FORMAT, "snapshot truncated");
   if (h.pos > 0) {
     CUDA_TRY(cudaSetDevice(s->device));
-    if (int rc = state_map(s, h.pos, 0)) return rc;
+    if (int rc = state_map(s, 0, h.pos, 0)) return rc;
     CUDA_TRY(cudaDeviceSynchronize());  // the table copy and steps in flight
     const size_t row = (size_t)h.pos * 2 * h.hd * h.elem_bytes;
     uint8_t* in = const_cast<uint8_t*>(static_cast<const uint8_t*>(src)) + sizeof h;

@@ -386,6 +386,9 @@ extern "C" int l3g_logprobs_status(l3g_logprobs* h, int32_t* err, int32_t* where
   return L3G_OK;
 }
 
+Result* chunk_attn_word(l3g_chunk_attn* h) { return h->d_res; }
+Result* logprobs_word(l3g_logprobs* h) { return h->d_res; }
+
 // ---------------------------------------------------------------------------
 // page copies
 // ---------------------------------------------------------------------------

@@ -152,6 +152,10 @@ struct l3g_kvpool {
   size_t page_bytes = 0;
   std::mutex mu;
   std::vector<int> free_pages;  // a stack of free page ids
+  std::vector<int> refs;        // states that map each page (shared pools)
+  std::vector<l3g_state*> members;  // the states on it (shared pools)
+  int* d_ids = nullptr;         // page lists of a copy (source, destination, rows)
+  int ids_cap = 0;
   int states = 0;               // states holding pages of it
   bool released = false;        // its owner freed it: destroyed with its last state
   bool priv = false;            // a state's private pool
@@ -166,16 +170,22 @@ struct l3g_state {
   int* d_pages = nullptr;      // page table [n_layers * local kv heads][pps] (device)
   std::vector<int> h_pages;    // its host copy; -1: not mapped
   int mapped = 0;              // logical pages [0, mapped) of every (layer, kv head) mapped
+  int high = 0;                // positions [0, high) have been written
   float* rope_cos = nullptr;
   float* rope_sin = nullptr;
   uint64_t serial = 0;
 };
 // The device view of a state's cache.
 KvMap state_kv(const l3g_state* s);  // l3g_model.cu
-// Maps pages for positions [0, n_pos) of every (layer, kv head), taking
-// them from the state's pool, and copies the new table entries to the
-// device on stream st (ordered before the kernels that use them).
-int state_map(l3g_state* s, int n_pos, cudaStream_t st);  // l3g_model.cu
+// Makes positions [pos0, n_pos) of every (layer, kv head) writable: maps pages
+// for positions [0, n_pos), taking them from the state's pool, gives the state
+// copies of its own of the pages of [pos0, n_pos) that others map too, and
+// copies the new table entries to the device on stream st (ordered before the
+// kernels that use them).  On failure nothing has changed.
+int state_map(l3g_state* s, int pos0, int n_pos, cudaStream_t st);  // l3g_model.cu
+// The error words of the serving operators' handles (l3g_ops.cu).
+Result* chunk_attn_word(l3g_chunk_attn* h);
+Result* logprobs_word(l3g_logprobs* h);
 
 // ---------------------------------------------------------------------------
 // workspace and the step graphs

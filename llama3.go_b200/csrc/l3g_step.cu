@@ -809,7 +809,7 @@ static int run_step(l3g_model* m, l3g_state* s, l3g_workspace* ws, int32_t token
   cudaGraphExec_t exec;
   int rc = get_graph(ws, s, variant, k, &exec);
   if (rc) return rc;
-  if ((rc = state_map(s, s->pos + 1, ws->stream))) return rc;
+  if ((rc = state_map(s, s->pos, s->pos + 1, ws->stream))) return rc;
   ws->h_io[0] = token;
   ws->h_io[1] = s->pos;
   ws->h_io[2] = 0;
@@ -890,7 +890,7 @@ extern "C" int l3g_decode_greedy(l3g_model* m, l3g_state* s, l3g_workspace* ws,
   cudaGraphExec_t exec;
   int rc = get_graph(ws, s, V_GREEDY_DEV, 0, &exec);
   if (rc) return rc;
-  if ((rc = state_map(s, s->pos + n, ws->stream))) return rc;
+  if ((rc = state_map(s, s->pos, s->pos + n, ws->stream))) return rc;
   cudaEvent_t e0, e1;
   CUDA_TRY(cudaEventCreate(&e0));
   CUDA_TRY(cudaEventCreate(&e1));
@@ -970,7 +970,7 @@ extern "C" int l3g_decode_sample(l3g_model* m, l3g_state* s, l3g_workspace* ws,
   cudaGraphExec_t exec;
   rc = get_graph(ws, s, V_SAMPLE_DEV, top_k, &exec);
   if (rc) return rc;
-  if ((rc = state_map(s, s->pos + n, ws->stream))) return rc;
+  if ((rc = state_map(s, s->pos, s->pos + n, ws->stream))) return rc;
   cudaEvent_t e0, e1;
   CUDA_TRY(cudaEventCreate(&e0));
   CUDA_TRY(cudaEventCreate(&e1));
@@ -1030,7 +1030,7 @@ extern "C" int l3g_profile_step(l3g_model* m, l3g_state* s, l3g_workspace* ws, i
   if (token < 0 || token >= m->hp.vocab_size)
     return l3g_fail(L3G_E_TOKEN, "token out of range: %d", token);
   CUDA_TRY(cudaSetDevice(m->device));
-  if (int rc0 = state_map(s, s->pos + 1, ws->stream)) return rc0;
+  if (int rc0 = state_map(s, s->pos, s->pos + 1, ws->stream)) return rc0;
   cudaEvent_t e0;
   CUDA_TRY(cudaEventCreate(&e0));
   ws->h_io[0] = token;
@@ -1083,7 +1083,7 @@ extern "C" int l3g_trace_step(l3g_model* m, l3g_state* s, l3g_workspace* ws, int
   cudaGraphExec_t exec;
   int rc = get_graph(ws, s, V_TRACE, 0, &exec);
   if (rc) return rc;
-  if ((rc = state_map(s, s->pos + 1, ws->stream))) return rc;
+  if ((rc = state_map(s, s->pos, s->pos + 1, ws->stream))) return rc;
   const int cnt = std::min<int>((int)ws->trace_kinds_graph.size(), kTraceCap);
   ws->h_io[0] = token;
   ws->h_io[1] = s->pos;

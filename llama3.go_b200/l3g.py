@@ -69,6 +69,13 @@ class TopKItem(C.Structure):
         return f"TopKItem(ID={self.ID}, Logit={self.Logit:.6g})"
 
 
+class _Score(C.Structure):
+    """l3g_score: what l3g_batch_extend writes per token."""
+    _fields_ = [("logprob", C.POINTER(C.c_float)), ("entropy", C.POINTER(C.c_float)),
+                ("rank", C.POINTER(C.c_int32)), ("top_k", C.c_int32),
+                ("top_ids", C.POINTER(C.c_int32)), ("top_logprobs", C.POINTER(C.c_float))]
+
+
 _lib = None
 _P = C.c_void_p
 
@@ -100,6 +107,11 @@ def lib():
         "l3g_kvpool_free": (None, [_P]),
         "l3g_kvpool_free_pages": (C.c_int, [_P, C.POINTER(C.c_int32)]),
         "l3g_state_new_in_pool": (C.c_int, [_P, _P, C.c_int32, C.POINTER(_P)]),
+        "l3g_state_fork": (C.c_int, [_P, C.c_int32, C.c_int32, C.POINTER(_P)]),
+        "l3g_state_trim": (C.c_int, [_P]),
+        "l3g_kvpool_compact": (C.c_int, [_P, C.POINTER(C.c_int32)]),
+        "l3g_batch_extend": (C.c_int, [_P, C.POINTER(_P), C.c_int32, C.POINTER(C.c_int32),
+                                       C.POINTER(C.c_int32), C.POINTER(C.c_int32), C.POINTER(_Score)]),
         "l3g_state_pages": (C.c_int, [_P, C.POINTER(C.c_int32)]),
         "l3g_state_pos": (C.c_int, [_P, C.POINTER(C.c_int32)]),
         "l3g_state_ctx_len": (C.c_int, [_P, C.POINTER(C.c_int32)]),
@@ -451,6 +463,17 @@ class State:
         _check(lib().l3g_state_pages(self._h, C.byref(v)))
         return v.value
 
+    def Fork(self, n_pos: int = -1, ctx_len: int = 0) -> "State":
+        """A new state that holds positions [0, n_pos) (-1: this state's own
+        position); in a shared pool the pages are shared until one writes."""
+        h = C.c_void_p()
+        _check(lib().l3g_state_fork(self._h, int(n_pos), int(ctx_len), C.byref(h)))
+        return State(self.model, h)
+
+    def Trim(self):
+        """Gives the pages behind the position back to the shared pool."""
+        _check(lib().l3g_state_trim(self._h))
+
     def Close(self):
         if self._h:
             lib().l3g_state_free(self._h)
@@ -474,6 +497,13 @@ class KvPool:
     def FreePages(self) -> int:
         v = C.c_int32()
         _check(lib().l3g_kvpool_free_pages(self._h, C.byref(v)))
+        return v.value
+
+    def Compact(self) -> int:
+        """Moves the pages in use to the lowest ids, each state's in order;
+        returns how many moved.  No step of the pool's states may run."""
+        v = C.c_int32()
+        _check(lib().l3g_kvpool_compact(self._h, C.byref(v)))
         return v.value
 
     def Close(self):
@@ -690,6 +720,41 @@ class Batch:
                                     nxt.ctypes.data_as(C.POINTER(C.c_int32)),
                                     _fptr(logits) if logits is not None else None))
         return (nxt, logits) if want_logits else nxt
+
+    def extend(self, states, chunks, targets=None, top_k: int = 0, score: bool = False):
+        """Each state ingests its chunk of given tokens (lists or arrays, some
+        may be empty).  With score (or targets) returns a dict of arrays over
+        all tokens, the chunks one after another: "entropy", "top_ids" and
+        "top_logprobs" [T][top_k], and with targets (per state, a token per
+        token of its chunk; -1: none) "logprob" and "rank"."""
+        n = len(states)
+        if len(chunks) != n or (targets is not None and [len(t) for t in targets] != [len(c) for c in chunks]):
+            raise L3GError(L3G_E_INVALID, "a chunk per state and a target per token")
+        arr = (C.c_void_p * n)(*[s._h.value if isinstance(s._h, C.c_void_p) else s._h for s in states])
+        i32 = C.POINTER(C.c_int32)
+
+        def flat(lists):
+            parts = [np.asarray(x, dtype=np.int32).reshape(-1) for x in lists]
+            return np.ascontiguousarray(np.concatenate(parts) if parts else np.empty(0, np.int32))
+        lens = np.asarray([len(c) for c in chunks], np.int32)
+        tok = flat(chunks)
+        tgt = flat(targets) if targets is not None else None
+        total = int(tok.size)
+        out, sc = None, None
+        if score or targets is not None:
+            out = {"entropy": np.empty(total, np.float32), "top_ids": np.empty((total, top_k), np.int32),
+                   "top_logprobs": np.empty((total, top_k), np.float32)}
+            sc = _Score(None, _fptr(out["entropy"]), None, top_k, out["top_ids"].ctypes.data_as(i32),
+                        _fptr(out["top_logprobs"]))
+            if tgt is not None:
+                out["logprob"] = np.empty(total, np.float32)
+                out["rank"] = np.empty(total, np.int32)
+                sc.logprob, sc.rank = _fptr(out["logprob"]), out["rank"].ctypes.data_as(i32)
+        _check(lib().l3g_batch_extend(self._h, C.cast(arr, C.POINTER(C.c_void_p)), n,
+                                      lens.ctypes.data_as(i32), tok.ctypes.data_as(i32),
+                                      tgt.ctypes.data_as(i32) if tgt is not None else None,
+                                      C.byref(sc) if sc is not None else None))
+        return out
 
     def Close(self):
         if self._h:

@@ -58,3 +58,29 @@ def test_descriptor_layout(l3g):
     assert l3g.CHUNK_SEQ.itemsize == 40
     assert [l3g.CHUNK_SEQ.fields[f][1] for f in ("pool", "pages", "n_pages", "pps", "q0", "n_q", "kv_len")] == \
         [0, 8, 16, 20, 24, 28, 32]
+
+
+def test_state_and_batch_null_arguments(l3g):
+    L = l3g.lib()
+    out = C.c_void_p()
+    n = C.c_int32()
+    assert L.l3g_state_fork(None, 0, 0, C.byref(out)) == l3g.L3G_E_INVALID
+    assert L.l3g_state_trim(None) == l3g.L3G_E_INVALID
+    assert L.l3g_kvpool_compact(None, C.byref(n)) == l3g.L3G_E_INVALID
+    assert L.l3g_batch_extend(None, None, 1, None, None, None, None) == l3g.L3G_E_INVALID
+    assert L.l3g_logprobs_status(None, None, None) == l3g.L3G_E_INVALID
+
+
+def test_compaction_moves(tmp_path):
+    """compact_plan's rounds put every page in its place through the scratch,
+    and no step reads what it writes (tests/pages_plan_check.cpp)."""
+    import os
+    import subprocess
+
+    from conftest import ROOT
+    exe = str(tmp_path / "pages_plan_check")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-I",
+                    os.path.join(ROOT, "llama3.go_b200", "csrc"),
+                    os.path.join(ROOT, "tests", "pages_plan_check.cpp"), "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stderr
