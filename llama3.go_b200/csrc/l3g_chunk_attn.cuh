@@ -33,9 +33,18 @@ constexpr int CHUNK_WARP_LOAD = CHUNK_WARP_OUT + CHUNK_OUT;
 constexpr int CHUNK_WARP_MMA = CHUNK_WARP_LOAD + CHUNK_LOAD;
 constexpr int CHUNK_WARPS = CHUNK_WARP_MMA + 1;
 constexpr int CHUNK_THREADS = 32 * CHUNK_WARPS;
-// registers per thread after the split; the block has 72 x 896 = 504 x 128
-constexpr int CHUNK_R_SOFT = 64, CHUNK_R_OUT = 168, CHUNK_R_REST = 40;
-static_assert(4 * CHUNK_R_SOFT + CHUNK_R_OUT + 2 * CHUNK_R_REST <= 504, "register split");
+// registers per thread after the split; the block has 72 x 896 = 504 x 128.  An
+// output thread holds HD of them.  The loaders of an f32 cache convert its
+// tiles, and its softmax threads have half as many keys
+__host__ __device__ constexpr int chunk_r_out(int hd) { return hd == 128 ? 168 : 104; }
+__host__ __device__ constexpr int chunk_r_soft(int es) { return es == 2 ? 64 : 56; }
+__host__ __device__ constexpr int chunk_r_rest(int hd, int es) {  // below the 72 of the launch
+  return hd == 128 ? (504 - 168 - 4 * chunk_r_soft(es)) / 2 : 64;
+}
+static_assert(4 * chunk_r_soft(2) + chunk_r_out(64) + 2 * chunk_r_rest(64, 2) <= 504 &&
+                  4 * chunk_r_soft(2) + chunk_r_out(128) + 2 * chunk_r_rest(128, 2) <= 504 &&
+                  4 * chunk_r_soft(4) + chunk_r_out(128) + 2 * chunk_r_rest(128, 4) <= 504,
+              "register split");
 constexpr int CHUNK_MIN_KEYS = 256;  // keys a CTA takes at least
 __host__ __device__ constexpr int chunk_min_tiles(int bn) { return CHUNK_MIN_KEYS / bn; }
 // tensor-memory columns: scores / weights of the two groups (at most 128
@@ -86,7 +95,8 @@ struct ChunkSmem {
   int n_tiles_lo, pad;
   long long begin, end;          // the CTA's range of the linear tile order
   long long unit0;               // first tile of the unit that holds `begin`
-  int s0, kvh0, rt0, per;
+  int s0, kvh0, rt0, pad0;
+  l3g_chunk_seq q0;              // its sequence's descriptor
   int bad[16];                   // segment + 1 whose pages are out of bounds
   float scale[32];               // f32 caches: 2^e of the items' tiles, item & 31
   ChunkCursor cur[CHUNK_WARPS];  // the warps' cursors, out of their registers
@@ -169,6 +179,11 @@ __device__ __forceinline__ int chunk_tiles(const l3g_chunk_seq& s, int tt, int r
   return see <= BN ? 1 : (int)((see + BN - 1) / BN);
 }
 
+// t * b / n for the ranges of the linear order (64-bit divisions take long)
+__device__ __forceinline__ long long chunk_cut(long long t, int b, int n) {
+  return t < 1 << 21 && n < 1 << 10 ? (long long)((uint32_t)t * (uint32_t)b / (uint32_t)n)
+                                    : t * b / n;
+}
 // The CTAs share the linear order (sequence, kv head, row tile, key tile) in
 // equal ranges; a row tile whose keys several CTAs hold is joined by
 // k_chunk_merge.  A cursor walks a CTA's range in segments, each the key tiles
@@ -189,7 +204,7 @@ __device__ __forceinline__ bool chunk_first(const ChunkArgs& a, const ChunkSmem*
   c.kvh = sh->kvh0;
   c.rt = sh->rt0;
   c.seg = 0;
-  c.q = a.seqs[c.s];
+  c.q = sh->q0;
   chunk_open<BN>(a, c, sh->end);
   return true;
 }
@@ -246,8 +261,8 @@ __device__ __forceinline__ void chunk_plan(const ChunkArgs& a, ChunkSmem* sh, in
     if (ctas > (long long)gridDim.x) ctas = gridDim.x;
     sh->begin = sh->end = 0;
     if ((long long)blockIdx.x < ctas) {
-      sh->begin = sum * blockIdx.x / ctas;
-      sh->end = sum * (blockIdx.x + 1) / ctas;
+      sh->begin = chunk_cut(sum, blockIdx.x, (int)ctas);
+      sh->end = chunk_cut(sum, blockIdx.x + 1, (int)ctas);
       int lo = 0, hi = a.n_seqs - 1;  // the last sequence that starts at or before it
       while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
@@ -256,8 +271,10 @@ __device__ __forceinline__ void chunk_plan(const ChunkArgs& a, ChunkSmem* sh, in
       }
       const l3g_chunk_seq q = a.seqs[lo];
       long long unit = sh->pre[lo];
-      const long long per = (sh->pre[lo + 1] - unit) / a.hkv;
-      const int kvh = (int)((sh->begin - unit) / per);
+      const long long all = sh->pre[lo + 1] - unit;  // a kv head's part of the sequence
+      const long long per = chunk_cut(all, 1, a.hkv);
+      const int kvh = all < 1 << 21 ? (int)((uint32_t)(sh->begin - unit) / (uint32_t)per)
+                                    : (int)((sh->begin - unit) / per);
       unit += per * kvh;
       int rt = 0;
       for (;; ++rt) {
@@ -265,6 +282,7 @@ __device__ __forceinline__ void chunk_plan(const ChunkArgs& a, ChunkSmem* sh, in
         if (sh->begin < unit + nk) break;
         unit += nk;
       }
+      sh->q0 = q;
       sh->s0 = lo;
       sh->kvh0 = kvh;
       sh->rt0 = rt;
@@ -276,8 +294,8 @@ __device__ __forceinline__ void chunk_plan(const ChunkArgs& a, ChunkSmem* sh, in
 // The CTA whose range holds linear tile t.
 __device__ __forceinline__ int chunk_owner(long long t, long long sum, int ctas) {
   int c = (int)(t * ctas / sum);
-  while (c + 1 < ctas && sum * (c + 1) / ctas <= t) ++c;
-  while (c > 0 && sum * c / ctas > t) --c;
+  while (c + 1 < ctas && chunk_cut(sum, c + 1, ctas) <= t) ++c;
+  while (c > 0 && chunk_cut(sum, c, ctas) > t) --c;
   return c;
 }
 
@@ -358,6 +376,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   uint8_t* ring = smem + chunk_ring_off();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tt = CHUNK_BM / a.group;
+  pdl_launch_dependents();
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
@@ -416,7 +435,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   bool ok = true;
 
   if (warp >= CHUNK_WARP_LOAD) {
-  regs_dec<CHUNK_R_REST>();
+  regs_dec<chunk_r_rest(HD, ES)>();
   if (warp < CHUNK_WARP_MMA) {
     // ---- loaders ----------------------------------------------------------
     // Warp lw brings the items lw, lw + NS, ... whole into slot lw: a tile whose
@@ -506,54 +525,79 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         if constexpr (ES == 4) {
           ok = chunk_wait(&sh->raw[lw], use & 1, sh, a, 41);
           if (!ok) break;
-          // the tile's scale, from its largest finite magnitude
-          float m = 0.0f;
-#pragma unroll 8
+          // the tile's scale, from its largest finite magnitude (a NaN loses
+          // against every number)
+          float m = 0.0f, m1 = 0.0f;
+#pragma unroll 4
           for (int e = lane; e < SLOT / 16; e += 32) {
             const float4 x = reinterpret_cast<const float4*>(dst)[e];
-            const float f[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int i2 = 0; i2 < 4; ++i2) {
-              const float v = fabsf(f[i2]);
-              m = v <= 3.4028235e38f ? fmaxf(m, v) : m;
-            }
+            m = max3(m, fabsf(x.x), fabsf(x.y));
+            m1 = max3(m1, fabsf(x.z), fabsf(x.w));
           }
-          const int e2 = exp_of(warp_max(m));  // it lands in [2^14, 2^15)
+          m = warp_max(fmaxf(m, m1));
+          if (m > 3.4028235e38f) {
+            m = 0.0f;
+#pragma unroll 1
+            for (int e = lane; e < SLOT / 4; e += 32) {
+              const float v = fabsf(reinterpret_cast<const float*>(dst)[e]);
+              if (v <= 3.4028235e38f) m = fmaxf(m, v);
+            }
+            m = warp_max(m);
+          }
+          const int e2 = exp_of(m);  // it lands in [2^14, 2^15)
           const float up = pow2i(14 - e2);
           if (lane == 0) sh->scale[it & 31] = 1.0f / up;
-          __syncwarp();
           // 8 lanes take a key's raw row (32 dims) or rows (64), 4 dims of
-          // each a lane, and put the two terms in their place
+          // each a lane, and put the two terms in their place; the rows of the
+          // four keys after them are on their way meanwhile.  (One warp, 64
+          // keys x 128 dims: 14000 cycles when each step waited for its loads.)
           constexpr int RAW = HD == 32 ? 1 : 2;  // raw rows that become hi and lo rows
-#pragma unroll 1
-          for (int p = 0; p < PANELS; p += RAW)
-#pragma unroll 4
-            for (int k0 = 0; k0 < BN; k0 += 4) {
-              const int k = k0 + kl;
-              uint8_t* row = dst + p * BOX;
-              float4 x[RAW];
+          const unsigned long long up2 = pk2(up, up), neg2 = pk2(-1.0f, -1.0f);
+          // Lane group kl takes the key k4 of eight, then the key k4 + 2: of keys
+          // 0, 1, 4, 5 (2, 3, 6, 7) the swizzle puts the halves of the rows that
+          // are written together in different banks.  The lane's pieces, read
+          // and written; bit 6 of the offset changes for the row's other half.
+          const int k4 = (kl & 1) + (kl >> 1) * 4;
+          const int rd = (cl ^ k4) << 4, wr = (((cl >> 1) ^ k4) << 4) + (cl & 1) * 8;
+          auto get = [&](const uint8_t* r0, float4 (&x)[RAW], int odd) {
 #pragma unroll
-              for (int r = 0; r < RAW; ++r)
-                x[r] = *reinterpret_cast<const float4*>(row + r * BOX + chunk_piece(128, k, cl));
-              __syncwarp();
+            for (int r = 0; r < RAW; ++r)
+              x[r] = *reinterpret_cast<const float4*>(r0 + r * BOX + (rd ^ odd));
+          };
+          auto put = [&](uint8_t* r0, const float4 (&x)[RAW], int odd) {
 #pragma unroll
-              for (int r = 0; r < RAW; ++r) {
-                uint2 hi, lo;
-                const float f0 = x[r].x * up, f1 = x[r].y * up, f2 = x[r].z * up, f3 = x[r].w * up;
-                hi.x = pack_h2(f0, f1);
-                hi.y = pack_h2(f2, f3);
-                const float2 b0 = unpack_h2(hi.x), b1 = unpack_h2(hi.y);
-                lo.x = pack_h2(f0 - b0.x, f1 - b0.y);
-                lo.y = pack_h2(f2 - b1.x, f3 - b1.y);
-                // dims 32 r + 4 cl .. of the 64 (or 32): 8 bytes of a 64-byte half row
-                const int at = r * 64 + cl * 8;
-                *reinterpret_cast<uint2*>(row + chunk_piece(128, k, at >> 4) + (at & 8)) = hi;
-                if constexpr (RAW == 2)
-                  *reinterpret_cast<uint2*>(row + BOX + chunk_piece(128, k, at >> 4) + (at & 8)) = lo;
-                else
-                  *reinterpret_cast<uint2*>(row + chunk_piece(128, k, (64 + at) >> 4) + (at & 8)) = lo;
-              }
+            for (int r = 0; r < RAW; ++r) {
+              const unsigned long long f0 = mul2(pk2(x[r].x, x[r].y), up2);
+              const unsigned long long f1 = mul2(pk2(x[r].z, x[r].w), up2);
+              uint2 hi, lo;
+              const float2 a0 = upk2(f0), a1 = upk2(f1);
+              hi.x = pack_h2(a0.x, a0.y);
+              hi.y = pack_h2(a1.x, a1.y);
+              const float2 b0 = unpack_h2(hi.x), b1 = unpack_h2(hi.y);
+              const float2 c0 = upk2(fma2(pk2(b0.x, b0.y), neg2, f0));
+              const float2 c1 = upk2(fma2(pk2(b1.x, b1.y), neg2, f1));
+              lo.x = pack_h2(c0.x, c0.y);
+              lo.y = pack_h2(c1.x, c1.y);
+              const int at = wr ^ odd ^ (r << 6);
+              *reinterpret_cast<uint2*>(r0 + at) = hi;
+              *reinterpret_cast<uint2*>(r0 + (RAW == 2 ? BOX + at : at ^ 64)) = lo;
             }
+          };
+          float4 xa[RAW], xb[RAW];
+#pragma unroll 1
+          for (int p = 0; p < PANELS; p += RAW) {
+            uint8_t* r0 = dst + p * BOX + k4 * 128;
+            get(r0, xa, 0);
+#pragma unroll 1
+            for (int k0 = 0; k0 < BN; k0 += 8, r0 += 1024) {
+              get(r0 + 256, xb, 32);
+              __syncwarp();
+              put(r0, xa, 0);
+              if (k0 + 8 < BN) get(r0 + 1024, xa, 0);
+              __syncwarp();
+              put(r0 + 256, xb, 32);
+            }
+          }
           fence_proxy_async_shared();
           __syncwarp();
           if (lane == 0) mbar_arrive(go);
@@ -653,7 +697,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   }
   } else if (warp >= CHUNK_WARP_OUT) {
     // ---- output -------------------------------------------------------------
-    regs_inc<CHUNK_R_OUT>();
+    regs_inc<chunk_r_out(HD)>();
     const uint32_t t_o = t_lane + CHUNK_T_O;
     float* tb = tbuf + warp * 32 * 17;
     int done = 0;  // tiles so far
@@ -810,7 +854,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     }
   } else {
     // ---- softmax ------------------------------------------------------------
-    regs_dec<CHUNK_R_SOFT>();
+    regs_dec<chunk_r_soft(ES)>();
     constexpr int KG = BN / 2;  // keys of a tile per thread
     constexpr int DG = HD / 4;  // dims of q per group
     const int g = warp >> 2, team = g & 1, half = g >> 1;
@@ -1033,64 +1077,50 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 
 // Joins the pieces of a row tile that several CTAs hold, in the order of the
 // CTAs: out = sum O_p 2^(m_p - M) / sum l_p 2^(m_p - M).  grid (CTAs of the
-// attention, row slices), 256 threads; a block takes its rows one by one, its
-// warps the row's pieces.
+// attention, CHUNK_BM / 8), 256 threads, a warp a row: its lanes take the
+// pieces' statistics side by side, then it adds the outputs, whose loads do not
+// wait for each other.  (A block a row at a time, with barriers, took 28 us for
+// 148 row tiles of two pieces.)  Launched early: it waits for the pieces itself.
 template <int HD>
 __global__ void __launch_bounds__(256) k_chunk_merge(const __grid_constant__ ChunkArgs a) {
-  __shared__ float sm_o[8][HD], sm_l[8], sm_m[8];
+  pdl_wait();
   const int* d = a.split + blockIdx.x * 8;
-  const int live = d[0];
-  if (live == 0) return;
-  const int c0 = d[1], c1 = blockIdx.x, n = c1 - c0 + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * 8 + warp;
+  if (r >= d[0]) return;  // (0: no split row tile ends in this CTA)
+  const int c0 = d[1], n = (int)blockIdx.x - c0 + 1;
   const l3g_chunk_seq q = a.seqs[d[2]];
-  const int kvh = d[3], tt = CHUNK_BM / a.group;
-  const long long row0 = (long long)q.q0 + (long long)d[4] * tt;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tt = CHUNK_BM / a.group;
   constexpr int V = HD / 32;
-  for (int r = blockIdx.y; r < live; r += gridDim.y) {
-    float M = -INFINITY, L = 0.0f, o[V];
-    bool bad = false;  // a maximum that is NaN marks a piece with a page outside its pool
+  float M = -INFINITY, L = 0.0f, o[V];
+  bool bad = false;  // a maximum that is NaN marks a piece with a page outside its pool
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = 0.0f;
-    for (int p = warp; p < n; p += 8) {
-      const size_t place = 2 * (size_t)(c0 + p) + (p == 0 ? 1 : 0);
-      const float m = a.part_ml[(place * CHUNK_BM + r) * 2];
-      const float l = a.part_ml[(place * CHUNK_BM + r) * 2 + 1];
-      bad |= m != m;
-      const float mn = fmaxf(M, m);
-      const float f = M == -INFINITY ? 0.0f : ex2(M - mn);
-      const float g = m == -INFINITY ? 0.0f : ex2(m - mn);
-      M = mn;
-      L = fmaf(L, f, l * g);
+  for (int i = 0; i < V; ++i) o[i] = 0.0f;
+  // (a piece that begins its row tile lies in its CTA's second place)
+  auto place = [&](int p) { return (2 * (size_t)(c0 + p) + (p == 0 ? 1 : 0)) * CHUNK_BM + r; };
+  for (int p0 = 0; p0 < n; p0 += 32) {
+    const int cnt = min(32, n - p0);
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (lane < cnt) ml = *reinterpret_cast<const float2*>(a.part_ml + place(p0 + lane) * 2);
+    bad = bad || __any_sync(0xffffffffu, ml.x != ml.x);
+    const float mn = fmaxf(M, warp_max(ml.x));
+    const float f = M == -INFINITY ? 0.0f : ex2(M - mn);
+    const float g = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mn);
+    M = mn;
+    L = fmaf(L, f, warp_sum(ml.y * g));
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        o[i] = fmaf(o[i], f, a.part_o[(place * CHUNK_BM + r) * HD + i * 32 + lane] * g);
-    }
-    if (lane == 0) {
-      sm_m[warp] = bad ? __int_as_float(0x7fc00000) : M;
-      sm_l[warp] = L;
-    }
+    for (int i = 0; i < V; ++i) o[i] *= f;
+#pragma unroll 4
+    for (int p = 0; p < cnt; ++p) {
+      const float gp = __shfl_sync(0xffffffffu, g, p);
+      const float* po = a.part_o + place(p0 + p) * HD;
 #pragma unroll
-    for (int i = 0; i < V; ++i) sm_o[warp][i * 32 + lane] = o[i];
-    __syncthreads();
-    if (threadIdx.x < HD) {
-      M = -INFINITY;
-      bad = false;
-      for (int w = 0; w < 8; ++w) {
-        bad |= sm_m[w] != sm_m[w];
-        M = fmaxf(M, sm_m[w]);
-      }
-      float O = 0.0f;
-      L = 0.0f;
-      for (int w = 0; w < 8; ++w) {
-        const float f = sm_m[w] == -INFINITY ? 0.0f : ex2(sm_m[w] - M);
-        L = fmaf(sm_l[w], f, L);
-        O = fmaf(sm_o[w][threadIdx.x], f, O);
-      }
-      if (!bad)
-        a.out[(row0 + r / a.group) * a.ldo + (size_t)(kvh * a.group + r % a.group) * HD +
-              threadIdx.x] = L > 0.0f ? O / L : L == 0.0f ? 0.0f : L;
+      for (int i = 0; i < V; ++i) o[i] = fmaf(po[i * 32 + lane], gp, o[i]);
     }
-    __syncthreads();
   }
+  if (bad) return;
+  float* out = a.out + ((long long)q.q0 + (long long)d[4] * tt + r / a.group) * a.ldo +
+               (size_t)(d[3] * a.group + r % a.group) * HD;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    out[i * 32 + lane] = L > 0.0f ? o[i] / L : L == 0.0f ? 0.0f : L;
 }

@@ -159,8 +159,17 @@ template <int HD, typename KT>
 static cudaError_t launch_chunk(const l3g_chunk_attn* h, const ChunkArgs& a, cudaStream_t st) {
   k_chunk_attention<HD, KT>
       <<<h->nsm, CHUNK_THREADS, chunk_smem_bytes(HD, (int)sizeof(KT)), st>>>(a);
-  k_chunk_merge<HD><<<dim3(h->nsm, 8), 256, 0, st>>>(a);
-  return cudaGetLastError();
+  if (const cudaError_t e = cudaGetLastError()) return e;
+  cudaLaunchAttribute at{};  // launched early: it waits for the pieces itself
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(h->nsm, CHUNK_BM / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_chunk_merge<HD>, a);
 }
 
 extern "C" int l3g_chunk_attn_run(l3g_chunk_attn* h, const l3g_chunk_seq* seqs, int32_t n_seqs,

@@ -97,7 +97,8 @@ template <int HD, typename KT>
 void run_chunk(const l3g::ChunkArgs& a, int grid) {
   simt::launch(dim3(grid), dim3(l3g::CHUNK_THREADS), l3g::chunk_smem_bytes(HD, (int)sizeof(KT)),
                [&] { l3g::k_chunk_attention<HD, KT>(a); });
-  simt::launch(dim3(grid, 8), dim3(256), 0, [&] { l3g::k_chunk_merge<HD>(a); }, true);
+  simt::launch(dim3(grid, l3g::CHUNK_BM / 8), dim3(256), 0, [&] { l3g::k_chunk_merge<HD>(a); },
+               true);
 }
 }  // namespace
 
