@@ -46,6 +46,10 @@ static_assert(4 * chunk_r_soft(2) + chunk_r_out(64) + 2 * chunk_r_rest(64, 2) <=
                   4 * chunk_r_soft(4) + chunk_r_out(128) + 2 * chunk_r_rest(128, 4) <= 504,
               "register split");
 constexpr int CHUNK_MIN_KEYS = 256;  // keys a CTA takes at least
+// what it costs to begin a row tile, in key tiles: q's terms, the first scores
+// and the last output, 10000 to 14000 cycles, where a tile takes 3000 to 4000.
+// (Ranges of equal tiles left SMs idle 40% of the time of 24 ragged sessions.)
+constexpr int CHUNK_OPEN = 4;
 __host__ __device__ constexpr int chunk_min_tiles(int bn) { return CHUNK_MIN_KEYS / bn; }
 // tensor-memory columns: scores / weights of the two groups (at most 128
 // each), q hi and lo (64 each), the tile output
@@ -74,8 +78,9 @@ struct ChunkArgs {
 
 // (see chunk_open)
 struct ChunkCursor {
-  long long pos, unit;  // next tile, first tile of its row tile
+  long long unit;       // where its row tile begins in the linear order
   int s, kvh, rt, seg;
+  int tiles;            // of the segments before
   l3g_chunk_seq q;      // the sequence's descriptor
   int nk, j0, j1;
 };
@@ -93,8 +98,8 @@ struct ChunkSmem {
   uint32_t tmem_base;
   int abort_flag;
   int n_tiles_lo, pad;
-  long long begin, end;          // the CTA's range of the linear tile order
-  long long unit0;               // first tile of the unit that holds `begin`
+  long long begin, end;          // the CTA's range of the linear order
+  long long unit0;               // where the row tile that holds `begin` begins
   int s0, kvh0, rt0, pad0;
   l3g_chunk_seq q0;              // its sequence's descriptor
   int bad[16];                   // segment + 1 whose pages are out of bounds
@@ -104,11 +109,12 @@ struct ChunkSmem {
   float gmax[2][2][2][CHUNK_BM]; // a tile's maxima [team][tile][key half]
   float m_tile[4][CHUNK_BM];     // what a tile's weights are relative to
   float m_team[2][CHUNK_BM], l_group[4][CHUNK_BM];  // a segment's statistics
-  long long pre[L3G_CHUNK_SEQS_MAX + 1];  // tiles before each sequence
+  long long pre[L3G_CHUNK_SEQS_MAX + 1];  // where each sequence begins in the linear order
 };
-constexpr int CHUNK_HEAD = 24 * 1024;
+constexpr int CHUNK_HEAD = 23 * 1024;
 static_assert(sizeof(ChunkSmem) <= CHUNK_HEAD, "chunk attention smem head");
-constexpr int CHUNK_TBUF = 32 * 17 * 4;  // a softmax or output warp's transposition buffer
+// transposition buffers of a softmax and of an output warp: rows of 16 floats
+constexpr int CHUNK_TBUF = 32 * 17 * 4, CHUNK_OBUF = 32 * 20 * 4;
 __host__ __device__ constexpr int chunk_slot_bytes(int hd, int es) {
   return chunk_bn(es) * hd * es;  // f16: one operand tile; f32: its hi and lo tiles
 }
@@ -119,18 +125,26 @@ __host__ __device__ constexpr int chunk_slots(int hd, int es) {
              : CHUNK_LOAD;
 }
 __host__ __device__ constexpr int chunk_ring_off() {
-  return (CHUNK_HEAD + (CHUNK_SOFT + CHUNK_OUT) * CHUNK_TBUF + 1023) / 1024 * 1024;
+  return (CHUNK_HEAD + CHUNK_SOFT * CHUNK_TBUF + CHUNK_OUT * CHUNK_OBUF + 1023) / 1024 * 1024;
 }
 // Operand tiles in shared memory: panels of up to 64 dims, [key][row bytes] with
 // the 16-byte pieces of a row swizzled by the key (the tensor core's 128-byte
 // and 64-byte swizzles), keys in groups of 8 one after another.  An f32 cache's
 // panel is fetched as two raw panels of 32 floats, and each key's two raw rows
-// become its hi and lo rows in place; with 32 dims a row holds hi, then lo.
+// become its hi and lo rows in place; with 32 dims a row holds hi, then lo.  The
+// lane that converts piece c of both raw rows, dims 4 c and 32 + 4 c on, leaves
+// them as piece c of the hi and the lo row: it overwrites only what it read, and
+// no lane waits for another.  So 64 dims of an f32 tile lie in the order of
+// chunk_dim, and so do q's, and the columns of the output.
 __host__ __device__ constexpr int chunk_row_bytes(int hd, int es) {
   return es == 2 && hd < 64 ? 64 : 128;
 }
 __host__ __device__ constexpr int chunk_box_cols(int hd, int es) {  // elements of a box's row
   return es == 4 ? 32 : hd < 64 ? 32 : 64;
+}
+// the dim at place `at` of an operand row
+__host__ __device__ constexpr int chunk_dim(int hd, int es, int at) {
+  return es == 2 || hd < 64 ? at : (at & ~63) + (at >> 2 & 1) * 32 + (at >> 3 & 7) * 4 + (at & 3);
 }
 // byte of 16-byte piece `piece` of key k in a panel of rows of rb bytes
 __host__ __device__ constexpr int chunk_piece(int rb, int k, int piece) {
@@ -184,37 +198,39 @@ __device__ __forceinline__ long long chunk_cut(long long t, int b, int n) {
   return t < 1 << 21 && n < 1 << 10 ? (long long)((uint32_t)t * (uint32_t)b / (uint32_t)n)
                                     : t * b / n;
 }
-// The CTAs share the linear order (sequence, kv head, row tile, key tile) in
-// equal ranges; a row tile whose keys several CTAs hold is joined by
-// k_chunk_merge.  A cursor walks a CTA's range in segments, each the key tiles
-// [j0, j1) of one row tile.
+// The CTAs share the linear order (sequence, kv head, row tile, key tile), in
+// which a row tile has CHUNK_OPEN places before its key tiles, in equal ranges;
+// a row tile whose keys several CTAs hold is joined by k_chunk_merge.  A cursor
+// walks a CTA's range in segments, each the key tiles [j0, j1) of one row tile.
 template <int BN>
-__device__ __forceinline__ void chunk_open(const ChunkArgs& a, ChunkCursor& c, long long end) {
+__device__ __forceinline__ bool chunk_open(const ChunkArgs& a, const ChunkSmem* sh,
+                                           ChunkCursor& c) {
   c.nk = chunk_tiles<BN>(c.q, CHUNK_BM / a.group, c.rt);
-  c.j0 = (int)(c.pos - c.unit);
-  c.j1 = (int)(end - c.unit < c.nk ? end - c.unit : c.nk);
+  const long long first = c.unit + CHUNK_OPEN, b = sh->begin - first, e = sh->end - first;
+  c.j0 = b > 0 ? (int)b : 0;
+  c.j1 = e < c.nk ? (int)e : c.nk;
+  return c.j1 > c.j0;
 }
 template <int BN>
 __device__ __forceinline__ bool chunk_first(const ChunkArgs& a, const ChunkSmem* sh,
                                             ChunkCursor& c) {
   if (sh->begin >= sh->end) return false;
-  c.pos = sh->begin;
   c.unit = sh->unit0;
   c.s = sh->s0;
   c.kvh = sh->kvh0;
   c.rt = sh->rt0;
   c.seg = 0;
+  c.tiles = 0;
   c.q = sh->q0;
-  chunk_open<BN>(a, c, sh->end);
-  return true;
+  return chunk_open<BN>(a, sh, c);
 }
 template <int BN>
 __device__ __forceinline__ bool chunk_next(const ChunkArgs& a, const ChunkSmem* sh,
                                            ChunkCursor& c) {
-  c.pos = c.unit + c.j1;
-  if (c.pos >= sh->end) return false;
-  c.unit = c.pos;  // a segment that ends before `end` ends its row tile
+  c.unit += CHUNK_OPEN + c.nk;
+  if (c.unit + CHUNK_OPEN >= sh->end) return false;  // the next key tile is not in the range
   ++c.seg;
+  c.tiles += c.j1 - c.j0;
   const int tt = CHUNK_BM / a.group;
   if (++c.rt >= (c.q.n_q + tt - 1) / tt) {
     c.rt = 0;
@@ -225,11 +241,16 @@ __device__ __forceinline__ bool chunk_next(const ChunkArgs& a, const ChunkSmem* 
       c.q = a.seqs[c.s];
     }
   }
-  chunk_open<BN>(a, c, sh->end);
-  return true;
+  return chunk_open<BN>(a, sh, c);
+}
+// CTAs that take part, of an order of `sum` places
+template <int BN>
+__device__ __forceinline__ int chunk_ctas(long long sum) {
+  constexpr int least = chunk_min_tiles(BN) + CHUNK_OPEN;
+  return sum > (long long)gridDim.x * least ? (int)gridDim.x : (int)((sum + least - 1) / least);
 }
 
-// Warp 0: the tiles of every sequence, then this CTA's range and where it starts.
+// Warp 0: the places of every sequence in the order, then this CTA's range and where it starts.
 template <int BN>
 __device__ __forceinline__ void chunk_plan(const ChunkArgs& a, ChunkSmem* sh, int lane) {
   const int tt = CHUNK_BM / a.group;
@@ -240,7 +261,8 @@ __device__ __forceinline__ void chunk_plan(const ChunkArgs& a, ChunkSmem* sh, in
     if (s < a.n_seqs) {
       const l3g_chunk_seq q = a.seqs[s];
       if (chunk_seq_ok(q, a.total_q)) {
-        for (int rt = 0; rt < (q.n_q + tt - 1) / tt; ++rt) n += chunk_tiles<BN>(q, tt, rt);
+        for (int rt = 0; rt < (q.n_q + tt - 1) / tt; ++rt)
+          n += CHUNK_OPEN + chunk_tiles<BN>(q, tt, rt);
         n *= a.hkv;
       } else if (blockIdx.x == 0) {
         report(a.res, ERR_SEQ, s);
@@ -257,12 +279,11 @@ __device__ __forceinline__ void chunk_plan(const ChunkArgs& a, ChunkSmem* sh, in
   if (lane == 0) sh->pre[a.n_seqs] = sum;
   __syncwarp();
   if (lane == 0) {
-    long long ctas = (sum + chunk_min_tiles(BN) - 1) / chunk_min_tiles(BN);
-    if (ctas > (long long)gridDim.x) ctas = gridDim.x;
+    const int ctas = chunk_ctas<BN>(sum);
     sh->begin = sh->end = 0;
-    if ((long long)blockIdx.x < ctas) {
-      sh->begin = chunk_cut(sum, blockIdx.x, (int)ctas);
-      sh->end = chunk_cut(sum, blockIdx.x + 1, (int)ctas);
+    if ((int)blockIdx.x < ctas) {
+      sh->begin = chunk_cut(sum, blockIdx.x, ctas);
+      sh->end = chunk_cut(sum, blockIdx.x + 1, ctas);
       int lo = 0, hi = a.n_seqs - 1;  // the last sequence that starts at or before it
       while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
@@ -278,9 +299,9 @@ __device__ __forceinline__ void chunk_plan(const ChunkArgs& a, ChunkSmem* sh, in
       unit += per * kvh;
       int rt = 0;
       for (;; ++rt) {
-        const int nk = chunk_tiles<BN>(q, tt, rt);
-        if (sh->begin < unit + nk) break;
-        unit += nk;
+        const int n = CHUNK_OPEN + chunk_tiles<BN>(q, tt, rt);
+        if (sh->begin < unit + n) break;
+        unit += n;
       }
       sh->q0 = q;
       sh->s0 = lo;
@@ -291,7 +312,7 @@ __device__ __forceinline__ void chunk_plan(const ChunkArgs& a, ChunkSmem* sh, in
   }
 }
 
-// The CTA whose range holds linear tile t.
+// The CTA whose range holds place t.
 __device__ __forceinline__ int chunk_owner(long long t, long long sum, int ctas) {
   int c = (int)(t * ctas / sum);
   while (c + 1 < ctas && chunk_cut(sum, c + 1, ctas) <= t) ++c;
@@ -299,7 +320,7 @@ __device__ __forceinline__ int chunk_owner(long long t, long long sum, int ctas)
   return c;
 }
 
-// o[d] = sum_j p_j V_j[d0 + d], d < 16, over the n keys of `rows` that a row
+// o[d] = sum_j p_j V_j[dim at place d0 + d], d < 16, over the n keys of `rows` that a row
 // sees, in fp32 from the cache itself: for a tile whose unseen keys hold a NaN
 // or an infinity, which the product would multiply by zero.  o is shared
 // memory of this thread's own; small loops, as it hardly ever runs.
@@ -316,7 +337,8 @@ __device__ __forceinline__ void chunk_row_slow(const KT* rows, int n, const floa
     for (int d = 0; d < HD; ++d) s = fmaf(q[d], (float)k[d], s);
     const float p = ex2(fmaf(s, scale, 13.0f - m));
 #pragma unroll 1
-    for (int d = 0; d < 16; ++d) o[d] = fmaf(p, (float)k[HD + d0 + d], o[d]);
+    for (int d = 0; d < 16; ++d)
+      o[d] = fmaf(p, (float)k[HD + chunk_dim(HD, (int)sizeof(KT), d0 + d)], o[d]);
   }
 }
 
@@ -528,11 +550,17 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           // the tile's scale, from its largest finite magnitude (a NaN loses
           // against every number)
           float m = 0.0f, m1 = 0.0f;
-#pragma unroll 4
-          for (int e = lane; e < SLOT / 16; e += 32) {
-            const float4 x = reinterpret_cast<const float4*>(dst)[e];
-            m = max3(m, fabsf(x.x), fabsf(x.y));
-            m1 = max3(m1, fabsf(x.z), fabsf(x.w));
+#pragma unroll 1
+          for (int e = lane; e < SLOT / 16; e += 256) {
+            float4 x[8];
+#pragma unroll
+            for (int i2 = 0; i2 < 8; ++i2)
+              x[i2] = reinterpret_cast<const float4*>(dst)[e + 32 * i2];
+#pragma unroll
+            for (int i2 = 0; i2 < 8; ++i2) {
+              m = max3(m, fabsf(x[i2].x), fabsf(x[i2].y));
+              m1 = max3(m1, fabsf(x[i2].z), fabsf(x[i2].w));
+            }
           }
           m = warp_max(fmaxf(m, m1));
           if (m > 3.4028235e38f) {
@@ -547,55 +575,55 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           const int e2 = exp_of(m);  // it lands in [2^14, 2^15)
           const float up = pow2i(14 - e2);
           if (lane == 0) sh->scale[it & 31] = 1.0f / up;
-          // 8 lanes take a key's raw row (32 dims) or rows (64), 4 dims of
-          // each a lane, and put the two terms in their place; the rows of the
-          // four keys after them are on their way meanwhile.  (One warp, 64
-          // keys x 128 dims: 14000 cycles when each step waited for its loads.)
-          constexpr int RAW = HD == 32 ? 1 : 2;  // raw rows that become hi and lo rows
           const unsigned long long up2 = pk2(up, up), neg2 = pk2(-1.0f, -1.0f);
-          // Lane group kl takes the key k4 of eight, then the key k4 + 2: of keys
-          // 0, 1, 4, 5 (2, 3, 6, 7) the swizzle puts the halves of the rows that
-          // are written together in different banks.  The lane's pieces, read
-          // and written; bit 6 of the offset changes for the row's other half.
-          const int k4 = (kl & 1) + (kl >> 1) * 4;
-          const int rd = (cl ^ k4) << 4, wr = (((cl >> 1) ^ k4) << 4) + (cl & 1) * 8;
-          auto get = [&](const uint8_t* r0, float4 (&x)[RAW], int odd) {
-#pragma unroll
-            for (int r = 0; r < RAW; ++r)
-              x[r] = *reinterpret_cast<const float4*>(r0 + r * BOX + (rd ^ odd));
+          // the two terms of four floats
+          auto split = [&](const float4& x, uint2& hi, uint2& lo) {
+            const unsigned long long f0 = mul2(pk2(x.x, x.y), up2);
+            const unsigned long long f1 = mul2(pk2(x.z, x.w), up2);
+            const float2 a0 = upk2(f0), a1 = upk2(f1);
+            hi.x = pack_h2(a0.x, a0.y);
+            hi.y = pack_h2(a1.x, a1.y);
+            const float2 b0 = unpack_h2(hi.x), b1 = unpack_h2(hi.y);
+            const float2 c0 = upk2(fma2(pk2(b0.x, b0.y), neg2, f0));
+            const float2 c1 = upk2(fma2(pk2(b1.x, b1.y), neg2, f1));
+            lo.x = pack_h2(c0.x, c0.y);
+            lo.y = pack_h2(c1.x, c1.y);
           };
-          auto put = [&](uint8_t* r0, const float4 (&x)[RAW], int odd) {
+          if constexpr (HD >= 64) {
+            // four keys' loads before the stores, which the compiler has to keep
+            // in their order: a step that waits for its own loads takes 175 cycles
+#pragma unroll 1
+            for (int p = 0; p < PANELS; p += 2) {
+              uint8_t* r0 = dst + p * BOX;
+#pragma unroll 1
+              for (int k0 = kl; k0 < BN; k0 += 16) {
+                float4 x[4], y[4];
 #pragma unroll
-            for (int r = 0; r < RAW; ++r) {
-              const unsigned long long f0 = mul2(pk2(x[r].x, x[r].y), up2);
-              const unsigned long long f1 = mul2(pk2(x[r].z, x[r].w), up2);
-              uint2 hi, lo;
-              const float2 a0 = upk2(f0), a1 = upk2(f1);
-              hi.x = pack_h2(a0.x, a0.y);
-              hi.y = pack_h2(a1.x, a1.y);
-              const float2 b0 = unpack_h2(hi.x), b1 = unpack_h2(hi.y);
-              const float2 c0 = upk2(fma2(pk2(b0.x, b0.y), neg2, f0));
-              const float2 c1 = upk2(fma2(pk2(b1.x, b1.y), neg2, f1));
-              lo.x = pack_h2(c0.x, c0.y);
-              lo.y = pack_h2(c1.x, c1.y);
-              const int at = wr ^ odd ^ (r << 6);
-              *reinterpret_cast<uint2*>(r0 + at) = hi;
-              *reinterpret_cast<uint2*>(r0 + (RAW == 2 ? BOX + at : at ^ 64)) = lo;
+                for (int i2 = 0; i2 < 4; ++i2) {
+                  const uint8_t* at = r0 + chunk_piece(128, k0 + 4 * i2, cl);
+                  x[i2] = *reinterpret_cast<const float4*>(at);
+                  y[i2] = *reinterpret_cast<const float4*>(at + BOX);
+                }
+#pragma unroll
+                for (int i2 = 0; i2 < 4; ++i2) {
+                  uint8_t* at = r0 + chunk_piece(128, k0 + 4 * i2, cl);
+                  uint2 h0, h1, l0, l1;
+                  split(x[i2], h0, l0);
+                  split(y[i2], h1, l1);
+                  *reinterpret_cast<uint4*>(at) = make_uint4(h0.x, h0.y, h1.x, h1.y);
+                  *reinterpret_cast<uint4*>(at + BOX) = make_uint4(l0.x, l0.y, l1.x, l1.y);
+                }
+              }
             }
-          };
-          float4 xa[RAW], xb[RAW];
+          } else {
 #pragma unroll 1
-          for (int p = 0; p < PANELS; p += RAW) {
-            uint8_t* r0 = dst + p * BOX + k4 * 128;
-            get(r0, xa, 0);
-#pragma unroll 1
-            for (int k0 = 0; k0 < BN; k0 += 8, r0 += 1024) {
-              get(r0 + 256, xb, 32);
+            for (int k = kl; k < BN; k += 4) {
+              const float4 x = *reinterpret_cast<const float4*>(dst + chunk_piece(128, k, cl));
               __syncwarp();
-              put(r0, xa, 0);
-              if (k0 + 8 < BN) get(r0 + 1024, xa, 0);
-              __syncwarp();
-              put(r0 + 256, xb, 32);
+              uint2 hi, lo;
+              split(x, hi, lo);
+              *reinterpret_cast<uint2*>(dst + chunk_piece(128, k, cl >> 1) + (cl & 1) * 8) = hi;
+              *reinterpret_cast<uint2*>(dst + chunk_piece(128, k, 4 + (cl >> 1)) + (cl & 1) * 8) = lo;
             }
           }
           fence_proxy_async_shared();
@@ -699,7 +727,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     // ---- output -------------------------------------------------------------
     regs_inc<chunk_r_out(HD)>();
     const uint32_t t_o = t_lane + CHUNK_T_O;
-    float* tb = tbuf + warp * 32 * 17;
+    float* tb = tbuf + CHUNK_SOFT * (CHUNK_TBUF / 4) + (warp - CHUNK_WARP_OUT) * (CHUNK_OBUF / 4);
     int done = 0;  // tiles so far
     // the next tile's product may overwrite the output: also from the start
     if (lane == 0) mbar_arrive(&sh->o_go[0]);
@@ -711,7 +739,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       // keys from the segment's first on that the row sees
       const int seen0 =
           live ? c.q.kv_len - c.q.n_q + c.rt * tt + (row * a.ginv >> 16) + 1 - c.j0 * BN : 0;
-      const int item0 = ES == 4 ? 2 * (int)(c.unit + c.j0 - sh->begin) : 0;
+      const int item0 = ES == 4 ? 2 * c.tiles : 0;
       unsigned long long o2[HD / 2];  // the output, dims 2 i and 2 i + 1
       float M = -INFINITY;            // what it is relative to
 #pragma unroll
@@ -751,9 +779,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                 uint32_t v[16];
                 tmem_get16(t_o + dc, v);
                 if (odd) {
-                  chunk_row_slow<HD, KT>(rows, in ? seen : 0, qrow, a.scale, mt, dc, tb + lane * 17);
+                  chunk_row_slow<HD, KT>(rows, in ? seen : 0, qrow, a.scale, mt, dc, tb + lane * 20);
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(tb[lane * 17 + i] / vs);
+                  for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(tb[lane * 20 + i] / vs);
                 }
                 __syncwarp();
                 tmem_st16(t_o + dc, v);
@@ -812,41 +840,43 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           a.part_ml[(place * CHUNK_BM + row) * 2] = bad ? __int_as_float(0x7fc00000) : M;
           a.part_ml[(place * CHUNK_BM + row) * 2 + 1] = L;
         }
-        // through shared memory, 16 dims at a time, four lanes a row
+        // through shared memory, 16 dims at a time, four lanes a row; the next
+        // segment's products wait for this, so all addresses are ready before
+        // and the stores of a step do not wait for each other (128 rows x 128
+        // dims in a rolled loop: 8000 to 14000 cycles)
         const int rl = lane >> 2, d4 = (lane & 3) * 4;
+        float* to[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = quarter * 32 + i * 8 + rl, tok = r * a.ginv >> 16;
+          to[i] = split ? a.part_o + (place * CHUNK_BM + r) * HD
+                        : a.out + (row0 + tok) * a.ldo + (size_t)(head0 + r - tok * a.group) * HD;
+          if (r >= live_rows || (bad && !split)) to[i] = nullptr;
+        }
 #pragma unroll
         for (int dc = 0; dc < HD; dc += 16) {
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 x = upk2(o2[dc / 2 + i]);
-            tb[lane * 17 + 2 * i] = x.x * inv;
-            tb[lane * 17 + 2 * i + 1] = x.y * inv;
+          for (int i = 0; i < 4; ++i) {
+            const float2 x = upk2(o2[dc / 2 + 2 * i]), y = upk2(o2[dc / 2 + 2 * i + 1]);
+            *reinterpret_cast<float4*>(tb + lane * 20 + 4 * i) =
+                make_float4(x.x * inv, x.y * inv, y.x * inv, y.y * inv);
           }
           __syncwarp();
-#pragma unroll 1
-          for (int i = 0; i < 32; i += 8) {
-            const int r = quarter * 32 + i + rl, tok = r * a.ginv >> 16;
-            const float* t = tb + (i + rl) * 17 + d4;
-            const float4 x = make_float4(t[0], t[1], t[2], t[3]);
-            if (r < live_rows) {
-              if (split)
-                *reinterpret_cast<float4*>(a.part_o + (place * CHUNK_BM + r) * HD + dc + d4) = x;
-              else if (!bad)
-                *reinterpret_cast<float4*>(a.out + (row0 + tok) * a.ldo +
-                                           (size_t)(head0 + r - tok * a.group) * HD + dc + d4) = x;
-            }
+          const int dim = chunk_dim(HD, ES, dc + d4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 x = *reinterpret_cast<const float4*>(tb + (i * 8 + rl) * 20 + d4);
+            if (to[i]) *reinterpret_cast<float4*>(to[i] + dim) = x;
           }
         }
       }
       if (warp == CHUNK_WARP_OUT && lane == 0 && split && c.j1 == c.nk) {
         // this CTA ends the row tile: what k_chunk_merge joins
         const long long sum = sh->pre[a.n_seqs];
-        long long ctas = (sum + chunk_min_tiles(BN) - 1) / chunk_min_tiles(BN);
-        if (ctas > (long long)gridDim.x) ctas = gridDim.x;
         int* d = a.split + blockIdx.x * 8;
         d[0] = live_rows;
-        d[1] = chunk_owner(c.unit, sum, (int)ctas);
+        d[1] = chunk_owner(c.unit + CHUNK_OPEN, sum, chunk_ctas<BN>(sum));
         d[2] = c.s;
         d[3] = c.kvh;
         d[4] = c.rt;
@@ -869,7 +899,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       // keys from the segment's first on that the row sees
       const int seen0 =
           live ? c.q.kv_len - c.q.n_q + c.rt * tt + (row * a.ginv >> 16) + 1 - c.j0 * BN : 0;
-      const int item0 = ES == 4 ? 2 * (int)(c.unit + c.j0 - sh->begin) : 0;
+      const int item0 = ES == 4 ? 2 * c.tiles : 0;
       // the last product that reads the q before this is complete
       if (t0 > 0) ok = wait(&sh->s_full[(t0 - 1) & 1], (t0 - 1) >> 1, 53);
       if (!ok) break;
@@ -879,7 +909,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         const long long row0 = (long long)c.q.q0 + c.rt * tt;
         const int head0 = c.kvh * a.group;
         // eight lanes read a row, four rows at a time, all in flight at once;
-        // group g takes the dims [g DG, g DG + DG); the terms go through shared
+        // group g takes the places [g DG, g DG + DG); the terms go through shared
         // memory to one row per lane
         const int rl4 = lane >> 3, l8 = lane & 7;
         constexpr int VL = DG / 8;  // floats of a row per lane
@@ -889,7 +919,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           const int r = quarter * 32 + i * 4 + rl4;
           const int tok = r * a.ginv >> 16;
           const float* src = a.q + (row0 + tok) * a.ldq +
-                             (size_t)(head0 + r - tok * a.group) * HD + g * DG + l8 * VL;
+                             (size_t)(head0 + r - tok * a.group) * HD +
+                             chunk_dim(HD, ES, g * DG + l8 * VL);
           if constexpr (VL == 4) {
             const float4 y = r < live_rows ? *reinterpret_cast<const float4*>(src)
                                            : make_float4(0.f, 0.f, 0.f, 0.f);
