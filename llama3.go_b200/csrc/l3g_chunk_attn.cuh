@@ -49,7 +49,7 @@ constexpr int CHUNK_MIN_KEYS = 256;  // keys a CTA takes at least
 // what it costs to begin a row tile, in key tiles: q's terms, the first scores
 // and the last output, 10000 to 14000 cycles, where a tile takes 3000 to 4000.
 // (Ranges of equal tiles left SMs idle 40% of the time of 24 ragged sessions.)
-constexpr int CHUNK_OPEN = 4;
+constexpr int CHUNK_OPEN = 6;
 __host__ __device__ constexpr int chunk_min_tiles(int bn) { return CHUNK_MIN_KEYS / bn; }
 // tensor-memory columns: scores / weights of the two groups (at most 128
 // each), q hi and lo (64 each), the tile output
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   const int tt = CHUNK_BM / a.group;
   pdl_launch_dependents();
 
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 32 * CHUNK_WARP_LOAD) {  // (while warp 0 plans)
     for (int i = 0; i < NS; ++i) {
       mbar_init(&sh->empty[i], 1);
       mbar_init(&sh->raw[i], 1);
@@ -426,7 +426,6 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     mbar_arrive(&sh->s_go[1]);
   }
   if (warp == 0) {
-    __syncwarp();
     chunk_plan<BN>(a, sh, lane);
   }
   if (warp == CHUNK_WARP_MMA) tmem_alloc(&sh->tmem_base, CHUNK_T_COLS);
