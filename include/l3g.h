@@ -548,8 +548,12 @@ void l3g_chunk_attn_free(l3g_chunk_attn *h);
  * 1 / sqrt(head_dim).  A descriptor outside its bounds (rows, kv_len, a page
  * id) is skipped, its rows left as they were (for a bad page: those of the
  * head's tokens that see it, at least), and noted for l3g_chunk_attn_status.
- * A NaN or an infinity in K or V gives NaN in the rows that see it and touches
- * no other. */
+ * A NaN in K or V, and an infinity in V, gives NaN in the rows that see it and
+ * touches no other; an infinite K counts as an infinite score, whose weight is
+ * zero if it is negative, or gives NaN.
+ * The products' operands keep 22 bits: q relative to a token and head's largest
+ * value, an f32 cache relative to the largest K (V) among the existing ones of
+ * 64 positions (64 i .. 64 i + 63), f16 caches exactly. */
 #define L3G_CHUNK_SEQS_MAX 512
 int l3g_chunk_attn_run(l3g_chunk_attn *h, const l3g_chunk_seq *seqs,
                        int32_t n_seqs, int32_t total_q, const float *q,
@@ -570,7 +574,8 @@ int l3g_chunk_attn_status(l3g_chunk_attn *h, int32_t *err, int32_t *where);
  * tokens of probability zero; a row of nothing else has entropy 0 and log
  * probabilities of -inf.  A row with a NaN or +inf has NaN for logprob, entropy
  * and top_logprobs; among its alternatives NaNs follow their sign bits beyond
- * the infinities, and its rank leaves NaNs out.  A target outside [0, vocab) is none: logprob NaN, rank -1.
+ * the infinities, and its rank leaves NaNs out.  A target outside
+ * [0, vocab) is none: logprob NaN, rank -1.
  * logprob and rank (with targets), entropy, top_ids and top_logprobs may be
  * NULL; top_k in [0, 64], at most vocab.  ld >= vocab. */
 typedef struct l3g_logprobs l3g_logprobs;

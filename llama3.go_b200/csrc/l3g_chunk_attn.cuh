@@ -8,6 +8,18 @@
 // one row tile of 128 rows (row r: token r / G, head r % G), which is the M of
 // both products; the cache is taken in tiles of CHUNK_BN keys.
 //
+// What bounds it (B200, 32 query and 8 kv heads of size 128).  f16 caches: the
+// tensor core needs 2048 cycles for a tile's two times two products, half its
+// rate for the one that a plain f16 attention takes, and the tiles follow each
+// other at 2700 to 3400, the time that two alternating tiles need for scores,
+// weights and output; 8 chunks of 1000 tokens after 7000: 2.1 to 2.3 ms, 430 to
+// 470 TFLOP/s at the 1.35 to 1.5 GHz that the power limit leaves.  64 decode
+// steps after 512 to 8192: 300 to 320 us, 4.0 to 4.2 TB/s; of a tile's 128 rows 4
+// are used, and one of the four schedulers does all of its exponentials.  f32
+// caches: the loaders' conversion, 5000 cycles per tile and warp; 24 ragged
+// sessions 194 us.  Short calls: the chain of latencies of a row tile, about
+// 10000 cycles (8 us) to its first output; one token 22 us.
+//
 // Precision.  q, out and the statistics are fp32; the products run on the f16
 // tensor cores.  An fp32 operand x goes in as two f16 terms, hi = f16(x) and
 // lo = f16(x - hi), after scaling by a power of two (exact, undone in fp32), so
@@ -20,8 +32,9 @@
 #pragma once
 
 constexpr int CHUNK_BM = 128;       // rows per tile: lanes of tensor memory
-// keys per tile (divides KV_PAGE): 128 of an f16 cache; 64 of an f32 cache,
-// whose tiles take twice the shared memory
+// keys per tile (divides KV_PAGE): 128 of an f16 cache (64: 64 decode steps in
+// 367 us instead of 316, 8 x 1000 tokens after 7000 in 2630 instead of 2300); 64
+// of an f32 cache, whose tiles take twice the shared memory
 __host__ __device__ constexpr int chunk_bn(int es) { return es == 2 ? 128 : 64; }
 // warps: 16 softmax (four groups of four: group g is team g & 1, key half
 // g >> 1), 4 output, 7 loaders, 1 that issues the products
@@ -45,10 +58,14 @@ static_assert(4 * chunk_r_soft(2) + chunk_r_out(64) + 2 * chunk_r_rest(64, 2) <=
                   4 * chunk_r_soft(2) + chunk_r_out(128) + 2 * chunk_r_rest(128, 2) <= 504 &&
                   4 * chunk_r_soft(4) + chunk_r_out(128) + 2 * chunk_r_rest(128, 4) <= 504,
               "register split");
-constexpr int CHUNK_MIN_KEYS = 256;  // keys a CTA takes at least
+// keys a CTA takes at least (one token after 300, f32: 128 keys 21.9 us, 256 keys
+// 22.4, 512 keys 26.6; long calls have more for each)
+constexpr int CHUNK_MIN_KEYS = 128;
 // what it costs to begin a row tile, in key tiles: q's terms, the first scores
 // and the last output, 10000 to 14000 cycles, where a tile takes 3000 to 4000.
-// (Ranges of equal tiles left SMs idle 40% of the time of 24 ragged sessions.)
+// (Ranges of equal tiles left SMs idle 40% of the time of 24 ragged sessions.
+// Weight 1 / 4 / 6: 24 ragged f32 sessions 216 / 193 / 194 us, 64 decode steps
+// 350 / 322 / 316, 7 x 300 tokens 44.8 / 45.0 / 43.3.)
 constexpr int CHUNK_OPEN = 6;
 __host__ __device__ constexpr int chunk_min_tiles(int bn) { return CHUNK_MIN_KEYS / bn; }
 // tensor-memory columns: scores / weights of the two groups (at most 128

@@ -256,16 +256,6 @@ extern "C" void l3g_logprobs_free(l3g_logprobs* h) {
   delete h;
 }
 
-// Values per thread of a slice (16 or 32: 4096 or 8192 values): the larger ones
-// where a row then needs no join, or where they still fill the CTAs that fit at
-// once (three per SM).
-static int logprob_slice(const l3g_logprobs* h, int n) {
-  const int big = 32 * LP_THREADS;
-  if (h->vocab <= 16 * LP_THREADS) return 16;
-  if (h->vocab <= big) return 32;
-  return (long long)n * ((h->vocab + big - 1) / big) >= 3LL * h->nsm ? 32 : 16;
-}
-
 // Kernel attributes, once per device, with that device current.
 static int logprob_setup() {
   static int rcs[64];
@@ -275,11 +265,8 @@ static int logprob_setup() {
     return l3g_fail(L3G_E_CUDA, "log probabilities set-up: no current device");
   int& rc = rcs[dev];
   std::call_once(onces[dev], [&rc] {
-    cudaError_t e = cudaFuncSetAttribute(
-        k_logprobs_part<16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, lp_smem(16));
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(k_logprobs_part<32, true>,
-                               cudaFuncAttributeMaxDynamicSharedMemorySize, lp_smem(32));
+    const cudaError_t e = cudaFuncSetAttribute(
+        k_logprobs_part<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, LP_SMEM);
     rc = e == cudaSuccess ? L3G_OK
                           : l3g_fail(L3G_E_CUDA, "log probabilities attributes: %s",
                                      cudaGetErrorString(e));
@@ -302,11 +289,7 @@ extern "C" int l3g_logprobs_new(int32_t max_rows, int32_t vocab, int32_t device,
   h->nsm = sm_count(dev);
   h->max_rows = max_rows;
   h->vocab = vocab;
-  size_t parts = 0;  // the most slices that any number of rows gets
-  for (int n = 1; n <= max_rows; n = n < 4 * h->nsm ? n + 1 : max_rows > n ? max_rows : n + 1) {
-    const int per = logprob_slice(h, n) * LP_THREADS;
-    parts = std::max(parts, (size_t)n * ((vocab + per - 1) / per));
-  }
+  const size_t parts = (size_t)max_rows * ((vocab + LP_SLICE - 1) / LP_SLICE);
   cudaError_t e = cudaMalloc(&h->part, parts * sizeof(float4));
   if (e == cudaSuccess)
     e = cudaMalloc(&h->part_k, parts * std::min(MAX_TOPK, vocab) * sizeof(uint64_t));
@@ -353,8 +336,7 @@ extern "C" int l3g_logprobs_run(l3g_logprobs* h, const float* logits, int64_t ld
   a.rank = rank;
   a.top_ids = top_ids;
   a.top_lp = top_logprobs;
-  const int e = logprob_slice(h, n);
-  a.slices = (h->vocab + e * LP_THREADS - 1) / (e * LP_THREADS);
+  a.slices = (h->vocab + LP_SLICE - 1) / LP_SLICE;
   a.part = h->part;
   a.part_k = h->part_k;
   const bool vec = !misaligned(logits, 16) && ld % 4 == 0;
@@ -362,10 +344,8 @@ extern "C" int l3g_logprobs_run(l3g_logprobs* h, const float* logits, int64_t ld
   a.res = h->d_res;
   a.wait_ns = WAIT_TIMEOUT_NS;
   const int grid = (int)std::min<long long>((long long)n * a.slices, 3LL * h->nsm);
-  if (e == 16 && vec) k_logprobs_part<16, true><<<grid, LP_THREADS, lp_smem(16), st>>>(a);
-  else if (e == 16) k_logprobs_part<16, false><<<grid, LP_THREADS, 0, st>>>(a);
-  else if (vec) k_logprobs_part<32, true><<<grid, LP_THREADS, lp_smem(32), st>>>(a);
-  else k_logprobs_part<32, false><<<grid, LP_THREADS, 0, st>>>(a);
+  if (vec) k_logprobs_part<true><<<grid, LP_THREADS, LP_SMEM, st>>>(a);
+  else k_logprobs_part<false><<<grid, LP_THREADS, 0, st>>>(a);
   CUDA_TRY(cudaGetLastError());
   if (a.slices > 1) {  // launched early: it waits for the slices itself
     cudaLaunchAttribute at{};
@@ -414,7 +394,7 @@ extern "C" int l3g_kv_copy_pages(const void* src_pool, int32_t n_src, void* dst_
   if (misaligned(src_pool, 16) || misaligned(dst_pool, 16) || misaligned(src, 4) ||
       misaligned(dst, 4) || misaligned(rows, 4) || misaligned(status, 4))
     return l3g_fail(L3G_E_INVALID, "pools must be 16-byte aligned, arrays 4-byte");
-  k_copy_pages<<<dim3(4, std::min(n, 65535)), 256, 0, (cudaStream_t)stream>>>(
+  k_copy_pages<<<dim3(COPY_SLICES, std::min(n, 65535)), 256, 0, (cudaStream_t)stream>>>(
       static_cast<const uint8_t*>(src_pool), n_src, static_cast<uint8_t*>(dst_pool), n_dst,
       row_bytes, src, dst, rows, n, status);
   CUDA_TRY(cudaGetLastError());

@@ -3,7 +3,11 @@
 #pragma once
 
 // Entry i copies rows [0, rows[i]) of page src[i] to page dst[i], 16 bytes a
-// thread and step.  grid (x: slices of an entry, y: entries).
+// thread and step.  grid (x: slices of an entry, y: entries).  Bound by memory:
+// every byte is read and written once.  2048 part-filled pages (269 MB moved) in
+// 48 us, 1500 whole ones (786 MB) in 127 us: 5.6 and 6.2 TB/s.  Slices of an
+// entry: one 54 and 139 us, four 48 and 127, eight 50 and 124.
+constexpr int COPY_SLICES = 4;
 static __global__ void k_copy_pages(const uint8_t* sp, int n_src, uint8_t* dp, int n_dst,
                                     int row_bytes, const int* src, const int* dst,
                                     const int* rows, int n, int* status) {
