@@ -740,9 +740,11 @@ extern "C" int l3g_state_fork(const l3g_state* src, int32_t n_pos, int32_t ctx,
   if (int rc = state_create(src->m, p->priv ? nullptr : p, ctx, &s)) return rc;
   const int heads = s->m->hp.n_layers * s->m->hkv_l;
   const int pages = (n_pos + KV_PAGE - 1) / KV_PAGE;
-  cudaError_t e = cudaSuccess;
+  cudaError_t e = cudaDeviceSynchronize();  // steps in flight on any stream
   int rc = L3G_OK;
-  if (p->priv) {  // its own pool: the rows are copied
+  if (e != cudaSuccess) {
+    // (reported below)
+  } else if (p->priv) {  // its own pool: the rows are copied
     std::vector<int> from, to, rows;
     for (int h = 0; h < heads; ++h)
       for (int j = 0; j < pages; ++j) {
@@ -750,10 +752,8 @@ extern "C" int l3g_state_fork(const l3g_state* src, int32_t n_pos, int32_t ctx,
         to.push_back(s->h_pages[(size_t)h * s->pps + j]);
         rows.push_back(std::min(KV_PAGE, n_pos - j * KV_PAGE));
       }
-    e = cudaDeviceSynchronize();  // steps in flight on any stream
-    if (e == cudaSuccess)
-      rc = copy_pages(s->pool, p->base, p->n_pages, s->pool->base, s->pool->n_pages, p->page_bytes,
-                      from, to, rows, nullptr);
+    rc = copy_pages(s->pool, p->base, p->n_pages, s->pool->base, s->pool->n_pages, p->page_bytes,
+                    from, to, rows, nullptr);
   } else {  // the pages are shared until one of the states writes to them
     {
       std::lock_guard<std::mutex> lk(p->mu);
