@@ -451,17 +451,22 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
 
-  // every warp walks the CTA's segments with a cursor of its own
+  // every warp walks the CTA's segments with a cursor of its own: lane 0 moves
+  // it between two __syncwarp, which order the lanes' reads of the old segment
+  // before the write and those of the new one behind it (a shuffle orders
+  // registers, not memory)
   ChunkCursor& c = sh->cur[warp];
   auto first = [&] {
     bool more = false;
     if (lane == 0) more = chunk_first<BN>(a, sh, c);
+    __syncwarp();
     return __shfl_sync(0xffffffffu, more ? 1 : 0, 0) != 0;
   };
   auto next = [&] {
     bool more = false;
     __syncwarp();
     if (lane == 0) more = chunk_next<BN>(a, sh, c);
+    __syncwarp();
     return __shfl_sync(0xffffffffu, more ? 1 : 0, 0) != 0;
   };
   auto wait = [&](uint64_t* b, int phase, int site) {
