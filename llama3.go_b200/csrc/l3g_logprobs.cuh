@@ -342,7 +342,9 @@ static __global__ void __launch_bounds__(LP_JOIN) k_logprobs_join(const LogprobA
       const float d = p.x == -INFINITY ? 0.0f : p.x - m;
       const float f = p.x == -INFINITY ? 1.0f : ex2(d * 1.44269504f);
       s = fmaf(p.y, f, s);
-      s1 = fmaf(fmaf(p.y, d, p.z), f, s1);
+      // (f is 0 from d = -150 on; S d of a slice of a mask's lowest values is
+      // beyond fp32's range, and -inf times that 0 would be NaN)
+      s1 = fmaf(fmaf(p.y, fmaxf(d, -1e30f), p.z), f, s1);
       before += __float_as_int(p.w);
     }
     s = warp_sum(s);

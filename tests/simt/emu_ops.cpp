@@ -67,6 +67,21 @@ inline void execute_mma(const TensorOp& op) {
 }
 }  // namespace simt
 
+inline unsigned __reduce_add_sync(unsigned mask, unsigned v) {
+  uint64_t all[32], s = 0;
+  simt::warp_exchange(mask, v, -1, "__reduce_add_sync", all);
+  for (uint64_t x : all) s += x;
+  return (unsigned)s;
+}
+inline int __ffs(unsigned v) { return __builtin_ffs((int)v); }
+inline unsigned long long atomicMax(unsigned long long* p, unsigned long long v) {
+  simt::yield();
+  const unsigned long long o = *p;
+  if (v > o) *p = v;
+  simt::made_progress();
+  return o;
+}
+
 #include "l3g.h"
 
 #define L3G_PTX_HEADER "simt_l3g_ptx.h"
@@ -77,6 +92,7 @@ namespace l3g {
 
 #include "l3g_chunk_attn.cuh"
 
+#include "l3g_logprobs.cuh"
 
 #include "l3g_pages.cuh"
 }  // namespace l3g
@@ -162,5 +178,69 @@ int emu_chunk_attention(const void* seqs, int n_seqs, int total_q, const float* 
   });
   for (void* p : scratch) simt::dfree(p);
   return rc;
+}
+
+// Log probabilities of n rows as l3g_logprobs_run launches them, on at most
+// max_grid CTAs; every pointer from emu_malloc (or null).
+int emu_logprobs(const float* x, long long ld, int n, int vocab, const int* targets, float* logprob,
+                 float* entropy, int* rank, int k, int* top_ids, float* top_lp, int vec, int max_grid,
+                 int* err) {
+  std::vector<void*> scratch;
+  auto dm = [&](size_t bytes) {
+    void* p = simt::dmalloc(bytes);
+    scratch.push_back(p);
+    return p;
+  };
+  const int rc = guarded_call([&] {
+    l3g::LogprobArgs a{};
+    a.x = x;
+    a.ld = ld;
+    a.n = n;
+    a.vocab = vocab;
+    a.k = k;
+    a.slices = (vocab + l3g::LP_SLICE - 1) / l3g::LP_SLICE;
+    a.targets = targets;
+    a.logprob = logprob;
+    a.entropy = entropy;
+    a.rank = rank;
+    a.top_ids = top_ids;
+    a.top_lp = top_lp;
+    a.res = static_cast<l3g::Result*>(dm(sizeof(l3g::Result)));
+    a.wait_ns = 1ull << 60;
+    a.part = static_cast<float4*>(dm((size_t)n * a.slices * sizeof(float4)));
+    a.part_k = static_cast<uint64_t*>(dm((size_t)n * a.slices * std::max(k, 1) * 8));
+    const dim3 grid(std::min(n * a.slices, max_grid));
+    // (a grid of one is not sequential by itself: its arrays are static all the same)
+    simt::seq_override() = true;
+    simt::seq_grid() = grid;
+    for (unsigned b = 0; b < grid.x; ++b) {
+      simt::seq_bidx() = uint3{b, 0, 0};
+      if (vec)
+        simt::launch(dim3(1), dim3(l3g::LP_THREADS), l3g::LP_SMEM,
+                     [&] { l3g::k_logprobs_part<true>(a); });
+      else
+        simt::launch(dim3(1), dim3(l3g::LP_THREADS), 0, [&] { l3g::k_logprobs_part<false>(a); });
+    }
+    simt::seq_grid() = dim3(n);
+    for (int r = 0; r < n && a.slices > 1; ++r) {
+      simt::seq_bidx() = uint3{(unsigned)r, 0, 0};
+      simt::launch(dim3(1), dim3(l3g::LP_JOIN), 0, [&] { l3g::k_logprobs_join(a); });
+    }
+    *err = a.res->err;
+  });
+  simt::seq_override() = false;
+  for (void* p : scratch) simt::dfree(p);
+  return rc;
+}
+
+// Page copies as l3g_kv_copy_pages launches them, on at most max_rows grid rows.
+int emu_copy_pages(const void* src_pool, int n_src, void* dst_pool, int n_dst, int row_bytes,
+                   const int* src, const int* dst, const int* rows, int n, int* status, int max_rows) {
+  return guarded_call([&] {
+    simt::launch(dim3(l3g::COPY_SLICES, std::min(n, max_rows)), dim3(256), 0, [&] {
+      l3g::k_copy_pages(static_cast<const uint8_t*>(src_pool), n_src, static_cast<uint8_t*>(dst_pool),
+                        n_dst, row_bytes, src, dst, rows, n, status);
+    });
+  });
 }
 }

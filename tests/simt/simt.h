@@ -513,15 +513,19 @@ inline void bar_sync(int id, int count) {
 // ---------------------------------------------------------------------------
 // mbarriers and bulk copies
 // ---------------------------------------------------------------------------
+// (in a sequential launch also a static shared array, which is a function static)
+inline bool mbar_place(const uint64_t* b) {
+  return (in_smem(cur()->blk, b, 8) || seq_override()) && !((uintptr_t)b & 7);
+}
 inline MBar& mbar(uint64_t* b, const char* what) {
-  if (!in_smem(cur()->blk, b, 8) || ((uintptr_t)b & 7))
+  if (!mbar_place(b))
     fail(std::string(what) + ": mbarrier outside this CTA's shared memory or unaligned");
   auto it = rt().mbars.find(b);
   if (it == rt().mbars.end()) fail(std::string(what) + ": mbarrier not initialised");
   return it->second;
 }
 inline void mbar_init(uint64_t* b, uint32_t count) {
-  if (!in_smem(cur()->blk, b, 8) || ((uintptr_t)b & 7)) fail("mbarrier.init outside shared memory");
+  if (!mbar_place(b)) fail("mbarrier.init outside shared memory");
   rt().mbars[b] = MBar{count, count, 0, 0};
 }
 inline void mbar_complete_if_done(MBar& m) {

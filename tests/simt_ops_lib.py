@@ -41,6 +41,9 @@ def lib():
         L.emu_chunk_attention.argtypes = [_P, C.c_int, C.c_int, _P, C.c_longlong, _P, C.c_longlong, C.c_int,
                                           C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int,
                                           C.POINTER(C.c_int), C.POINTER(C.c_int)]
+        L.emu_logprobs.argtypes = [_P, C.c_longlong, C.c_int, C.c_int, _P, _P, _P, _P, C.c_int, _P, _P, C.c_int,
+                                   C.c_int, C.POINTER(C.c_int)]
+        L.emu_copy_pages.argtypes = [_P, C.c_int, _P, C.c_int, C.c_int, _P, _P, _P, C.c_int, _P, C.c_int]
         _lib = L
     return _lib
 
@@ -105,3 +108,47 @@ def chunk_attention(cache, chunks, heads, q, grid=3, scale=None, layer=0, seed=N
     finally:
         for b in pool_d + [table_d, qd, out, sd]:
             b.free()
+
+
+def logprobs(x, targets, k, ld=None, shift=0, grid=5, seed=None):
+    """Runs the kernels on rows of logits, `shift` floats behind a 16-byte
+    boundary at row stride ld; returns a dict of lp, ent, rank, ids, tlp."""
+    L = lib()
+    L.emu_schedule(0 if seed is None else 1, seed or 0, 40)
+    n, v = x.shape
+    ld = ld or v
+    buf = np.full(shift + n * ld, np.nan, np.float32)
+    buf[shift:].reshape(n, ld)[:, :v] = x
+    xd, td = Dev(buf), Dev(np.asarray(targets, np.int32))
+    o = {"lp": Dev(np.full(n, 7, np.float32)), "ent": Dev(np.full(n, 7, np.float32)),
+         "rank": Dev(np.full(n, 7, np.int32)), "ids": Dev(np.full((n, max(k, 1)), 7, np.int32)),
+         "tlp": Dev(np.full((n, max(k, 1)), 7, np.float32))}
+    err = C.c_int()
+    try:
+        check(L.emu_logprobs(xd.ptr + 4 * shift, ld, n, v, td.ptr, o["lp"].ptr, o["ent"].ptr, o["rank"].ptr, k,
+                             o["ids"].ptr, o["tlp"].ptr, int(shift % 4 == 0 and ld % 4 == 0), grid, C.byref(err)))
+        if err.value:
+            raise RuntimeError(f"device check {err.value}")
+        return {a: b.read() for a, b in o.items()}
+    finally:
+        for b in [xd, td, *o.values()]:
+            b.free()
+
+
+def copy_pages(src_pool, dst_pool, src, dst, rows=None, max_rows=65535):
+    """k_copy_pages between two pools [pages][PAGE][row bytes] (uint8), None for
+    dst_pool: within one; returns (the destination pool, status)."""
+    L = lib()
+    L.emu_schedule(0, 0, 40)
+    i32 = np.int32
+    a = Dev(src_pool)
+    b = a if dst_pool is None else Dev(dst_pool)
+    sd, dd, st = Dev(np.asarray(src, i32)), Dev(np.asarray(dst, i32)), Dev(np.zeros(2, i32))
+    rd = None if rows is None else Dev(np.asarray(rows, i32))
+    try:
+        check(L.emu_copy_pages(a.ptr, a.shape[0], b.ptr, b.shape[0], a.shape[2], sd.ptr, dd.ptr,
+                               rd.ptr if rd else None, len(src), st.ptr, max_rows))
+        return b.read(), tuple(st.read())
+    finally:
+        for x in {id(y): y for y in (a, b, sd, dd, st, rd) if y}.values():
+            x.free()
