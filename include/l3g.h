@@ -548,9 +548,10 @@ void l3g_chunk_attn_free(l3g_chunk_attn *h);
  * 1 / sqrt(head_dim).  A descriptor outside its bounds (rows, kv_len, a page
  * id) is skipped, its rows left as they were (for a bad page: those of the
  * head's tokens that see it, at least), and noted for l3g_chunk_attn_status.
- * A NaN in K or V, and an infinity in V, gives NaN in the rows that see it and
- * touches no other; an infinite K counts as an infinite score, whose weight is
- * zero if it is negative, or gives NaN.
+ * A NaN in q gives NaN in its row, one in K or V in the rows that see it, and
+ * touches no other.  An infinite K makes a score infinite: -inf weighs nothing
+ * (a token with no other score gets zeros), +inf gives NaN.  An infinity in q
+ * gives NaN, one in V that infinity or NaN in the rows that see it.
  * The products' operands keep 22 bits: q relative to a token and head's largest
  * value, an f32 cache relative to the largest K (V) among the existing ones of
  * 64 positions (64 i .. 64 i + 63), f16 caches exactly. */

@@ -352,7 +352,7 @@ __device__ __forceinline__ void chunk_row_slow(const KT* rows, int n, const floa
     float s = 0.0f;
 #pragma unroll 1
     for (int d = 0; d < HD; ++d) s = fmaf(q[d], (float)k[d], s);
-    const float p = ex2(fmaf(s, scale, 13.0f - m));
+    const float p = ex2(fmaf(s, scale, 13.0f - (m == -INFINITY ? 0.0f : m)));
 #pragma unroll 1
     for (int d = 0; d < 16; ++d)
       o[d] = fmaf(p, (float)k[HD + chunk_dim(HD, (int)sizeof(KT), d0 + d)], o[d]);
@@ -375,6 +375,83 @@ __device__ __forceinline__ float2 unpack_h2(uint32_t u) {
   return __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+// The rows of a quarter (bits of `rows`, a lane each) whose sum over the segment
+// came out as NaN, once more in fp32 from the cache itself, by the whole warp: a
+// lane a key for the scores, HD / 32 dims a lane for the output.  An infinity of
+// K comes as NaN from two-term operands (its lo term, or a q term that is zero
+// or has the other sign), where a score of -inf weighs nothing.  A row with a
+// score that is NaN or +inf, or with a q that is not finite, stays NaN, as it
+// was written.  It hardly ever runs (32 rows over 128 Ki keys: below the waits'
+// bound, which the other warps' waits for this one have to keep).
+template <int HD, typename KT>
+__device__ __forceinline__ void chunk_rows_again(const ChunkArgs& a, const ChunkCursor& c,
+                                                 uint32_t rows, int quarter, int lane, bool split,
+                                                 size_t place) {
+  constexpr int V = HD / 32, BN = chunk_bn((int)sizeof(KT));
+  const int tt = CHUNK_BM / a.group;
+  const int* pages = c.q.pages + ((size_t)a.layer * a.hkv + c.kvh) * c.q.pps;
+#pragma unroll 1
+  for (; rows; rows &= rows - 1) {
+    const int row = quarter * 32 + __ffs(rows) - 1, tok = row * a.ginv >> 16;
+    const long long at = (long long)c.q.q0 + (long long)c.rt * tt + tok;
+    const int head = c.kvh * a.group + row - tok * a.group;
+    const float* q = a.q + at * a.ldq + (size_t)head * HD;
+    const int end = min(c.j1 * BN, c.q.kv_len - c.q.n_q + c.rt * tt + tok + 1);
+    float M = -INFINITY, L = 0.0f, o[V];
+    bool good = true;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      o[i] = 0.0f;
+      good = good && fabsf(q[lane * V + i]) <= 3.4028235e38f;
+    }
+    good = __all_sync(0xffffffffu, good);
+#pragma unroll 1
+    for (int kb = c.j0 * BN; kb < end && good; kb += 32) {  // (32 divides a page)
+      const int page = pages[kb / KV_PAGE], cnt = min(32, end - kb);
+      good = page >= 0 && page < c.q.n_pages;
+      if (!good) break;
+      const KT* cells = reinterpret_cast<const KT*>(c.q.pool) +
+                        ((size_t)page * KV_PAGE + (kb & (KV_PAGE - 1))) * 2 * HD;
+      float s = -INFINITY;
+      if (lane < cnt) {
+        const KT* k = cells + (size_t)lane * 2 * HD;
+        float d4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int d = 0; d < HD; d += 4)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d4[i] = fmaf(q[d + i], (float)k[d + i], d4[i]);
+        s = ((d4[0] + d4[1]) + (d4[2] + d4[3])) * a.scale;
+      }
+      good = __all_sync(0xffffffffu, s < INFINITY);
+      if (!good) break;
+      const float mn = fmaxf(M, warp_max(s)), mu = mn == -INFINITY ? 0.0f : mn;
+      const float f = M == -INFINITY ? 0.0f : ex2(M - mu);
+      const float p = ex2(s - mu + 13.0f);  // (the scale of the segment's weights)
+      L = fmaf(L, f, warp_sum(p));
+      M = mn;
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] *= f;
+#pragma unroll 8
+      for (int j = 0; j < cnt; ++j) {
+        const float pj = __shfl_sync(0xffffffffu, p, j);
+        const KT* v = cells + (size_t)j * 2 * HD + HD + lane * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = fmaf(pj, (float)v[i], o[i]);
+      }
+    }
+    if (!good) continue;
+    float* to = split ? a.part_o + (place * CHUNK_BM + row) * HD
+                      : a.out + at * a.ldo + (size_t)head * HD;
+    const float inv = split ? 1.0f : L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+#pragma unroll
+    for (int i = 0; i < V; ++i) to[lane * V + i] = o[i] * inv;
+    if (split && lane == 0) {
+      a.part_ml[(place * CHUNK_BM + row) * 2] = M;
+      a.part_ml[(place * CHUNK_BM + row) * 2 + 1] = L;
+    }
+  }
+}
+
 // 2^e as a float, e in [-126, 127]
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 // the exponent of the largest magnitude m, limited so that pow2i takes the
@@ -890,6 +967,11 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             const float4 x = *reinterpret_cast<const float4*>(tb + (i * 8 + rl) * 20 + d4);
             if (to[i]) *reinterpret_cast<float4*>(to[i] + dim) = x;
           }
+        }
+        const uint32_t again = __ballot_sync(0xffffffffu, live && !bad && L != L);
+        if (again) {
+          __syncwarp();  // (over what other lanes have written)
+          chunk_rows_again<HD, KT>(a, c, again, quarter, lane, split, place);
         }
       }
       if (warp == CHUNK_WARP_OUT && lane == 0 && split && c.j1 == c.nk) {
