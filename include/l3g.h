@@ -459,7 +459,8 @@ int l3g_batch_step(l3g_batch *b, l3g_state *const *states, int32_t n,
  * the token that follows, the entropy, and the top_k alternatives.  score's
  * arrays are HOST arrays of T entries ([T][top_k] the last two), each nullable.
  * One GPU (no tensor parallelism).  On failure the states' positions are those
- * of the last completed pass.  (The reference ingests one session's tokens one
+ * of the last completed pass; a call whose pools have too few pages for all its
+ * sessions (L3G_E_CTX) takes none, as l3g_batch_step.  (The reference ingests one session's tokens one
  * by one and keeps the last token's logits, main.go:276-286.) */
 typedef struct {
   float *logprob;

@@ -2,8 +2,6 @@
 // snapshots.
 #include "l3g_rt.h"
 
-#include "l3g_pages_plan.h"
-
 // ---------------------------------------------------------------------------
 // tiled Q8_0 matrices
 // ---------------------------------------------------------------------------
@@ -485,17 +483,6 @@ static void pool_destroy(l3g_kvpool* p) {
   delete p;
 }
 
-// A state lets go of a page (the pool is locked): free once no state maps it.
-static void page_drop(l3g_kvpool* p, int id) {
-  if (--p->refs[id] == 0) p->free_pages.push_back(id);
-}
-static int page_take(l3g_kvpool* p) {
-  const int id = p->free_pages.back();
-  p->free_pages.pop_back();
-  p->refs[id] = 1;
-  return id;
-}
-
 // A state leaves its pool: the pages that no other state maps go back on the
 // free list; a released (or private) pool without states is destroyed.
 static void pool_leave(l3g_kvpool* p, l3g_state* s) {
@@ -504,7 +491,7 @@ static void pool_leave(l3g_kvpool* p, l3g_state* s) {
     std::lock_guard<std::mutex> lk(p->mu);
     if (!p->priv) {
       for (int id : s->h_pages)
-        if (id >= 0) page_drop(p, id);
+        if (id >= 0) p->drop(id);
       p->members.erase(std::remove(p->members.begin(), p->members.end(), s), p->members.end());
     }
     --p->states;
@@ -550,55 +537,66 @@ static int copy_pages(l3g_kvpool* via, const uint8_t* src_base, int n_src, uint8
   return L3G_OK;
 }
 
-int state_map(l3g_state* s, int pos0, int n_pos, cudaStream_t st) {
-  const int need = std::min(s->pps, (n_pos + KV_PAGE - 1) / KV_PAGE);
-  const int heads = s->m->hp.n_layers * s->m->hkv_l;
-  l3g_kvpool* p = s->pool;
-  int first = s->mapped, last = need;  // the table columns that change
-  if (!p->priv) {
-    std::lock_guard<std::mutex> lk(p->mu);
-    // pages of the range that other states map too
-    std::vector<size_t> shared;
-    for (int j = pos0 / KV_PAGE; j < std::min(need, s->mapped); ++j)
-      for (int h = 0; h < heads; ++h)
-        if (p->refs[s->h_pages[(size_t)h * s->pps + j]] > 1) shared.push_back((size_t)h * s->pps + j);
-    const size_t want = shared.size() + (size_t)heads * std::max(0, need - s->mapped);
-    if (p->free_pages.size() < want)
-      return l3g_fail(L3G_E_CTX, "KV pool exhausted: %zu free pages, %zu needed for position %d",
-                      p->free_pages.size(), want, n_pos - 1);
-    if (!shared.empty()) {
-      std::vector<int> src, dst, rows;
-      for (size_t e : shared) {
-        src.push_back(s->h_pages[e]);
-        dst.push_back(page_take(p));
-        const int j = (int)(e % s->pps);
-        rows.push_back(std::max(0, std::min(KV_PAGE, s->high - j * KV_PAGE)));
-      }
-      if (int rc = copy_pages(p, p->base, p->n_pages, p->base, p->n_pages, p->page_bytes, src, dst,
-                              rows, st)) {
-        for (int id : dst) page_drop(p, id);
-        return rc;
-      }
-      for (size_t i = 0; i < shared.size(); ++i) {
-        page_drop(p, src[i]);
-        s->h_pages[shared[i]] = dst[i];
-        first = std::min(first, (int)(shared[i] % s->pps));
-      }
-      last = std::max(last, std::min(need, s->mapped));
-    }
-    for (int j = s->mapped; j < need; ++j)
-      for (int h = 0; h < heads; ++h) s->h_pages[(size_t)h * s->pps + j] = page_take(p);
+int states_map(const std::vector<MapSpan>& spans, cudaStream_t st) {
+  std::vector<l3g_kvpool*> pools;  // locked in the order of their addresses
+  for (const MapSpan& x : spans)
+    if (!x.s->pool->priv) pools.push_back(x.s->pool);  // (a private pool's are mapped)
+  std::sort(pools.begin(), pools.end());
+  pools.erase(std::unique(pools.begin(), pools.end()), pools.end());
+  std::vector<std::unique_lock<std::mutex>> locks;
+  for (l3g_kvpool* p : pools) locks.emplace_back(p->mu);
+  // the books first: all of it, or none
+  std::vector<PageMapping> maps(spans.size());
+  auto undo = [&](size_t n) {
+    while (n-- > 0)
+      if (!spans[n].s->pool->priv) pages_unmap(*spans[n].s->pool, *spans[n].s, maps[n]);
+  };
+  for (size_t i = 0; i < spans.size(); ++i) {
+    l3g_state* s = spans[i].s;
+    if (s->pool->priv ||
+        pages_map(*s->pool, *s, KV_PAGE, spans[i].pos0, spans[i].n_pos, s->high, maps[i]))
+      continue;
+    size_t want = maps[i].want;
+    for (size_t j = 0; j < i; ++j)
+      if (spans[j].s->pool == s->pool) want += maps[j].want;
+    undo(i);
+    return l3g_fail(L3G_E_CTX, "KV pool exhausted: %zu free pages, %zu needed for position %d",
+                    s->pool->free_pages.size(), want, spans[i].n_pos - 1);
   }
-  s->high = std::max(s->high, n_pos);
-  if (first >= last) return L3G_OK;
-  // the new entries of every (layer, kv head): one 2-D copy (pageable
-  // source: staged before the call returns)
-  CUDA_TRY(cudaMemcpy2DAsync(s->d_pages + first, (size_t)s->pps * sizeof(int),
-                             s->h_pages.data() + first, (size_t)s->pps * sizeof(int),
-                             (size_t)(last - first) * sizeof(int), (size_t)heads,
-                             cudaMemcpyHostToDevice, st));
-  s->mapped = std::max(s->mapped, need);
+  // then the copies and the new entries of every (layer, kv head): one 2-D copy
+  // a state (pageable source: staged before the call returns)
+  int rc = L3G_OK;
+  for (l3g_kvpool* p : pools) {
+    std::vector<int> src, dst, rows;
+    for (size_t i = 0; i < spans.size(); ++i)
+      if (spans[i].s->pool == p) {
+        src.insert(src.end(), maps[i].src.begin(), maps[i].src.end());
+        dst.insert(dst.end(), maps[i].dst.begin(), maps[i].dst.end());
+        rows.insert(rows.end(), maps[i].rows.begin(), maps[i].rows.end());
+      }
+    if (!rc)
+      rc = copy_pages(p, p->base, p->n_pages, p->base, p->n_pages, p->page_bytes, src, dst, rows, st);
+  }
+  for (size_t i = 0; i < spans.size() && !rc; ++i) {
+    l3g_state* s = spans[i].s;
+    const PageMapping& m = maps[i];
+    if (m.first >= m.last) continue;
+    const cudaError_t e = cudaMemcpy2DAsync(
+        s->d_pages + m.first, (size_t)s->pps * sizeof(int), s->h_pages.data() + m.first,
+        (size_t)s->pps * sizeof(int), (size_t)(m.last - m.first) * sizeof(int), (size_t)s->heads(),
+        cudaMemcpyHostToDevice, st);
+    if (e != cudaSuccess) rc = l3g_fail(L3G_E_CUDA, "KV page table: %s", cudaGetErrorString(e));
+  }
+  if (rc) {
+    undo(spans.size());
+    return rc;
+  }
+  for (const MapSpan& x : spans) x.s->high = std::max(x.s->high, x.n_pos);
   return L3G_OK;
+}
+
+int state_map(l3g_state* s, int pos0, int n_pos, cudaStream_t st) {
+  return states_map({{s, pos0, n_pos}}, st);
 }
 
 extern "C" int l3g_kvpool_page_bytes(const l3g_model* m, uint64_t* bytes) {
@@ -790,7 +788,7 @@ extern "C" int l3g_state_trim(l3g_state* s) {
   for (int h = 0; h < heads; ++h)
     for (int j = keep; j < s->mapped; ++j) {
       int& id = s->h_pages[(size_t)h * s->pps + j];
-      page_drop(p, id);
+      p->drop(id);
       id = -1;
     }
   s->mapped = keep;  // (the device table's entries behind it are not read)

@@ -1,5 +1,98 @@
-// The moves of a pool compaction (l3g_kvpool_compact), shared by the host
-// runtime and its CPU check.  Plain C++, no CUDA API.
+// The bookkeeping of a KV pool's pages, shared by the host runtime and its CPU
+// checks: which pages states map, what a step has to map or copy before it
+// writes, and the moves of a compaction.  Plain C++, no CUDA API.
+#pragma once
+
+#include <algorithm>
+#include <utility>
+#include <vector>
+
+namespace l3g {
+
+// Pages of a shared pool.  Under the pool's lock.
+struct PageBook {
+  std::vector<int> free_pages;  // a stack of free page ids
+  std::vector<int> refs;        // states that map each page
+  int take() {
+    const int id = free_pages.back();
+    free_pages.pop_back();
+    refs[id] = 1;
+    return id;
+  }
+  void drop(int id) {  // free once no state maps it
+    if (--refs[id] == 0) free_pages.push_back(id);
+  }
+};
+
+// A state's page table: entry [h * pps + j] is page j of (layer, kv head) h.
+struct PageTable {
+  int pps = 0;               // pages per (layer, kv head)
+  std::vector<int> h_pages;  // -1: not mapped
+  int mapped = 0;            // pages [0, mapped) of every (layer, kv head) are mapped
+  int heads() const { return pps ? (int)(h_pages.size() / pps) : 0; }
+};
+
+// One state's part of making positions writable, and what undoes it.
+struct PageMapping {
+  size_t want = 0;                // pages that it takes
+  int mapped0 = 0;                // the table's `mapped` before
+  int first = 0, last = 0;        // the table's columns that changed
+  std::vector<size_t> entries;    // entries whose page others map too, and their
+  std::vector<int> src, dst;      // page, the state's own copy of it
+  std::vector<int> rows;          // and the rows of it that have been written
+};
+
+// Makes positions [pos0, n_pos) of table t writable: maps pages for positions
+// [0, n_pos), and replaces those of [pos0, n_pos) that other states map too by
+// pages of its own (whose copies, m.src to m.dst, the caller makes; positions
+// [0, high) have been written).  False where the pool has too few free pages:
+// then nothing but m.want has changed.
+inline bool pages_map(PageBook& book, PageTable& t, int page, int pos0, int n_pos, int high,
+                      PageMapping& m) {
+  const int heads = t.heads(), need = std::min(t.pps, (n_pos + page - 1) / page);
+  m = PageMapping{};
+  m.mapped0 = m.first = t.mapped;
+  m.last = std::max(t.mapped, need);
+  for (int j = pos0 / page; j < std::min(need, t.mapped); ++j)
+    for (int h = 0; h < heads; ++h)
+      if (book.refs[t.h_pages[(size_t)h * t.pps + j]] > 1)
+        m.entries.push_back((size_t)h * t.pps + j);
+  m.want = m.entries.size() + (size_t)heads * (m.last - t.mapped);
+  if (book.free_pages.size() < m.want) return false;
+  for (size_t e : m.entries) {
+    const int j = (int)(e % t.pps);
+    m.src.push_back(t.h_pages[e]);
+    m.dst.push_back(book.take());
+    m.rows.push_back(std::max(0, std::min(page, high - j * page)));
+    m.first = std::min(m.first, j);
+    t.h_pages[e] = m.dst.back();
+    book.drop(m.src.back());
+  }
+  for (int j = t.mapped; j < need; ++j)
+    for (int h = 0; h < heads; ++h) t.h_pages[(size_t)h * t.pps + j] = book.take();
+  t.mapped = m.last;
+  return true;
+}
+
+// Takes a pages_map back.  Several are taken back in the reverse order: then
+// pool and tables are what they were, the order of the free pages too.
+inline void pages_unmap(PageBook& book, PageTable& t, const PageMapping& m) {
+  const int heads = t.heads();
+  for (int j = t.mapped - 1; j >= m.mapped0; --j)
+    for (int h = heads - 1; h >= 0; --h) {
+      int& id = t.h_pages[(size_t)h * t.pps + j];
+      book.drop(id);
+      id = -1;
+    }
+  t.mapped = m.mapped0;
+  for (size_t i = m.entries.size(); i-- > 0;) {
+    t.h_pages[m.entries[i]] = m.src[i];
+    ++book.refs[m.src[i]];
+    book.drop(m.dst[i]);
+  }
+}
+
+// The moves of a pool compaction (l3g_kvpool_compact).
 //
 // `order` lists the pages in use in the order they shall have: order[t] is the
 // page that becomes page t.  Pages move through a scratch of `batch` pages, a
@@ -9,13 +102,6 @@
 //      places that step 1 emptied (outside the targets),
 //   3. scratch to the targets.
 // No copy of a step reads what another copy of it writes.
-#pragma once
-
-#include <utility>
-#include <vector>
-
-namespace l3g {
-
 struct CompactRound {
   std::vector<std::pair<int, int>> out;   // page -> scratch page
   std::vector<std::pair<int, int>> away;  // page -> page

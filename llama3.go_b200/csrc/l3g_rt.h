@@ -32,6 +32,7 @@
 #include "l3g.h"
 #include "l3g_internal.h"
 #include "l3g_kernels.cuh"
+#include "l3g_pages_plan.h"
 
 using namespace l3g;
 
@@ -144,15 +145,13 @@ struct l3g_model {
 // position grows and give them back when freed.  A state made by
 // l3g_state_new has a private pool holding exactly its pages (freed with
 // it); l3g_kvpool_new makes a pool several states share.
-struct l3g_kvpool {
+struct l3g_kvpool : PageBook {  // (its pages' counts: shared pools only)
   l3g_model* m = nullptr;
   int device = 0;
   uint8_t* base = nullptr;
   int n_pages = 0;
   size_t page_bytes = 0;
   std::mutex mu;
-  std::vector<int> free_pages;  // a stack of free page ids
-  std::vector<int> refs;        // states that map each page (shared pools)
   std::vector<l3g_state*> members;  // the states on it (shared pools)
   int* d_ids = nullptr;         // page lists of a copy (source, destination, rows)
   int ids_cap = 0;
@@ -161,15 +160,12 @@ struct l3g_kvpool {
   bool priv = false;            // a state's private pool
 };
 
-struct l3g_state {
+struct l3g_state : PageTable {
   l3g_model* m = nullptr;
   int device = 0;
   int ctx = 0, pos = 0;
   l3g_kvpool* pool = nullptr;  // where its pages live
-  int pps = 0;                 // pages per (layer, kv head): ceil(ctx / KV_PAGE)
   int* d_pages = nullptr;      // page table [n_layers * local kv heads][pps] (device)
-  std::vector<int> h_pages;    // its host copy; -1: not mapped
-  int mapped = 0;              // logical pages [0, mapped) of every (layer, kv head) mapped
   int high = 0;                // positions [0, high) have been written
   float* rope_cos = nullptr;
   float* rope_sin = nullptr;
@@ -177,12 +173,18 @@ struct l3g_state {
 };
 // The device view of a state's cache.
 KvMap state_kv(const l3g_state* s);  // l3g_model.cu
-// Makes positions [pos0, n_pos) of every (layer, kv head) writable: maps pages
-// for positions [0, n_pos), taking them from the state's pool, gives the state
-// copies of its own of the pages of [pos0, n_pos) that others map too, and
-// copies the new table entries to the device on stream st (ordered before the
-// kernels that use them).  On failure nothing has changed.
-int state_map(l3g_state* s, int pos0, int n_pos, cudaStream_t st);  // l3g_model.cu
+// Makes positions [pos0, n_pos) of every (layer, kv head) of each state writable:
+// maps pages for positions [0, n_pos), taking them from the states' pools, gives
+// each state copies of its own of the pages of [pos0, n_pos) that others map too
+// (one launch a pool), and copies the new table entries to the device on stream
+// st (ordered before the kernels that use them).  All or none: on failure nothing
+// has changed.
+struct MapSpan {
+  l3g_state* s;
+  int pos0, n_pos;
+};
+int states_map(const std::vector<MapSpan>& spans, cudaStream_t st);  // l3g_model.cu
+int state_map(l3g_state* s, int pos0, int n_pos, cudaStream_t st);   // of one state
 // The error words of the serving operators' handles (l3g_ops.cu).
 Result* chunk_attn_word(l3g_chunk_attn* h);
 Result* logprobs_word(l3g_logprobs* h);
