@@ -175,7 +175,8 @@ int l3g_state_new_in_pool(l3g_model *m, l3g_kvpool *pool, int32_t ctx_len,
                           l3g_state **out);
 int l3g_state_pages(const l3g_state *s, int32_t *mapped);
 /* A new state that holds src's positions [0, n_pos) (n_pos < 0: its own
- * position) and continues from there; ctx_len <= 0 means src's.  In a shared
+ * position; at most those that it has ingested, or restored, since it was last
+ * trimmed) and continues from there; ctx_len <= 0 means src's.  In a shared
  * pool the two share the pages: nothing is copied until one of them writes to
  * a page that the other maps too, which then gives the writer a copy of its
  * own (a step that finds no free page for it fails with L3G_E_CTX).  A state

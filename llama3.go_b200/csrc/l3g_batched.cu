@@ -484,7 +484,7 @@ extern "C" int l3g_prefill_batched(l3g_model* m, l3g_state* s, l3g_workspace* ws
       return l3g_fail(L3G_E_DEVICE, "device check failed: code %d at site %d (%s)", code, where,
                       code == ERR_TIMEOUT ? "bounded wait ran out" : "bad input");
     }
-    s->pos += P;
+    s->advance(P);
   }
   return L3G_OK;
 }
@@ -840,7 +840,7 @@ extern "C" int l3g_batch_step(l3g_batch* b, l3g_state* const* states, int32_t n,
   }
   for (int i = 0; i < n; ++i) {
     next_tokens[i] = b->h_out[i].token;
-    states[i]->pos++;
+    states[i]->advance(1);
   }
   return L3G_OK;
 }
@@ -1085,7 +1085,7 @@ extern "C" int l3g_batch_extend(l3g_batch* b, l3g_state* const* states, int32_t 
       return l3g_fail(L3G_E_DEVICE, "device check failed: code %d at site %d (%s)", code, where,
                       code == ERR_TIMEOUT ? "bounded wait ran out" : "bad input");
     }
-    for (const auto& s : took) states[s.first]->pos += s.second;
+    for (const auto& s : took) states[s.first]->advance(s.second);
     t0 += P;
   }
   return L3G_OK;

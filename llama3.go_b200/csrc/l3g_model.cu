@@ -591,7 +591,6 @@ int states_map(const std::vector<MapSpan>& spans, cudaStream_t st) {
     undo(spans.size());
     return rc;
   }
-  for (const MapSpan& x : spans) x.s->high = std::max(x.s->high, x.n_pos);
   return L3G_OK;
 }
 
@@ -994,7 +993,7 @@ extern "C" int l3g_state_restore(l3g_state* s, const void* src, uint64_t bytes) 
         if (int rc = copy_rows(s, l, k, 0, h.pos, in + ((size_t)l * h.hkv_l + k) * row, false))
           return rc;
   }
-  s->pos = h.pos;
+  s->pos = s->high = h.pos;
   return L3G_OK;
 }
 

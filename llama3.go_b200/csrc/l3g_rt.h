@@ -166,7 +166,12 @@ struct l3g_state : PageTable {
   int ctx = 0, pos = 0;
   l3g_kvpool* pool = nullptr;  // where its pages live
   int* d_pages = nullptr;      // page table [n_layers * local kv heads][pps] (device)
-  int high = 0;                // positions [0, high) have been written
+  int high = 0;                // positions [0, high) have been ingested
+  // n positions more, by a step that has ended well
+  void advance(int n) {
+    pos += n;
+    high = std::max(high, pos);
+  }
   float* rope_cos = nullptr;
   float* rope_sin = nullptr;
   uint64_t serial = 0;

@@ -824,7 +824,7 @@ static int run_step(l3g_model* m, l3g_state* s, l3g_workspace* ws, int32_t token
                     code == ERR_TIMEOUT ? "bounded wait ran out" : "bad input");
   }
   ws->logits_valid = variant != V_PREFILL;
-  s->pos++;
+  s->advance(1);
   return L3G_OK;
 }
 
@@ -919,7 +919,7 @@ extern "C" int l3g_decode_greedy(l3g_model* m, l3g_state* s, l3g_workspace* ws,
   }
   if (device_ms) *device_ms = ms;
   ws->logits_valid = true;
-  s->pos += n;
+  s->advance(n);
   return L3G_OK;
 }
 
@@ -1015,7 +1015,7 @@ extern "C" int l3g_decode_sample(l3g_model* m, l3g_state* s, l3g_workspace* ws,
   *n_out = kept;
   if (device_ms) *device_ms = ms;
   ws->logits_valid = kept == n;
-  s->pos += kept < n ? kept + 1 : n;
+  s->advance(kept < n ? kept + 1 : n);
   return L3G_OK;
 }
 
@@ -1065,7 +1065,7 @@ extern "C" int l3g_profile_step(l3g_model* m, l3g_state* s, l3g_workspace* ws, i
     return l3g_fail(L3G_E_DEVICE, "device check failed during profiling");
   }
   *n = std::min(cnt, *n);
-  s->pos++;
+  s->advance(1);
   return L3G_OK;
 }
 
@@ -1103,7 +1103,7 @@ extern "C" int l3g_trace_step(l3g_model* m, l3g_state* s, l3g_workspace* ws, int
                       cudaMemcpyDeviceToHost));
   for (int i = 0; i < out_n; ++i) kinds[i] = ws->trace_kinds_graph[i];
   *n = out_n;
-  s->pos++;
+  s->advance(1);
   return L3G_OK;
 }
 

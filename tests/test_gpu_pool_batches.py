@@ -81,3 +81,35 @@ def test_two_forks_of_a_batch_share_one_copy(gpu_lib):
         own.Close()
     for x in (a, f, batch, pool, m):
         x.Close()
+
+
+def test_a_fork_holds_only_what_its_source_ingested(gpu_lib):
+    """Positions that were mapped, sampled past a stop token or lie behind a
+    restored snapshot are none of the session's."""
+    import synthetic
+    cfg, m, h = _load(gpu_lib)
+    ids = synthetic.prompt_ids(cfg, 300, seed=3)
+    ws = m.NewWorkspace(512, 40)
+    pool = m.NewKvPool(8 * h)
+    a = m.NewStateInPool(pool, 512)
+    m.Prefill(a, ids[:20], ws)
+    m.DecodeSample(a, int(ids[20]), 6, ws, top_k=40, temperature=0.8, seed=5)
+    a.Pos = 20
+    a.Fork(26).Close()  # back, but they have been ingested
+    with pytest.raises(gpu_lib.L3GError, match="fork at position 27"):
+        a.Fork(27)
+    b = m.NewStateInPool(pool, 512)
+    m.Prefill(b, ids[:20], ws)
+    m.DecodeSample(b, int(ids[20]), 6, ws, top_k=40, temperature=0.8, seed=5, stop_ids=list(range(cfg.vocab)))
+    assert b.Pos < 26
+    with pytest.raises(gpu_lib.L3GError, match="fork at position 26"):
+        b.Fork(26)
+    snap = b.Snapshot()
+    m.Prefill(a, ids[20:300], ws)
+    a.Restore(snap)
+    assert a.Pos == b.Pos
+    with pytest.raises(gpu_lib.L3GError, match=f"fork at position {b.Pos + 1}"):
+        a.Fork(b.Pos + 1)
+    a.Fork(b.Pos).Close()
+    for x in (a, b, ws, pool, m):
+        x.Close()
