@@ -708,7 +708,7 @@ extern "C" int l3g_batch_step(l3g_batch* b, l3g_state* const* states, int32_t n,
   const float scale = (float)(1.0 / sqrt((double)hd));
   std::vector<MapSpan> spans;  // each session's page for this step's position
   for (int i = 0; i < n; ++i) spans.push_back({states[i], states[i]->pos, states[i]->pos + 1});
-  if (int rc = states_map(spans, st)) return rc;
+  if (int rc = states_map(std::move(spans), st)) return rc;
   CUDA_TRY(cudaMemcpyAsync(b->d_seq, b->h_seq, (size_t)n * sizeof(SeqInfo),
                            cudaMemcpyHostToDevice, st));
   k_bd_embed<<<dim3((ne + 255) / 256, n), 256, 0, st>>>(m->emb, hp.vocab_size, ne, b->d_seq, b->x,
@@ -1020,7 +1020,7 @@ extern "C" int l3g_batch_extend(l3g_batch* b, l3g_state* const* states, int32_t 
   std::vector<MapSpan> spans;  // each session's pages
   for (int i = 0; i < n; ++i)
     if (n_tokens[i] > 0) spans.push_back({states[i], states[i]->pos, states[i]->pos + n_tokens[i]});
-  if (int rc = states_map(spans, st)) return rc;
+  if (int rc = states_map(std::move(spans), st)) return rc;
   int seq = 0, seq_done = 0;  // the next token: session and place in its chunk
   for (long long t0 = 0; t0 < total;) {
     const int P = (int)std::min<long long>(EXT_CAP, total - t0);

@@ -537,10 +537,16 @@ static int copy_pages(l3g_kvpool* via, const uint8_t* src_base, int n_src, uint8
   return L3G_OK;
 }
 
-int states_map(const std::vector<MapSpan>& spans, cudaStream_t st) {
+int states_map(std::vector<MapSpan> spans, cudaStream_t st) {
+  // (a private pool's pages are all mapped, by its state alone)
+  spans.erase(std::remove_if(spans.begin(), spans.end(),
+                             [](const MapSpan& x) {
+                               return pages_ready(*x.s, KV_PAGE, x.pos0, x.n_pos);
+                             }),
+              spans.end());
+  if (spans.empty()) return L3G_OK;
   std::vector<l3g_kvpool*> pools;  // locked in the order of their addresses
-  for (const MapSpan& x : spans)
-    if (!x.s->pool->priv) pools.push_back(x.s->pool);  // (a private pool's are mapped)
+  for (const MapSpan& x : spans) pools.push_back(x.s->pool);
   std::sort(pools.begin(), pools.end());
   pools.erase(std::unique(pools.begin(), pools.end()), pools.end());
   std::vector<std::unique_lock<std::mutex>> locks;
@@ -548,14 +554,11 @@ int states_map(const std::vector<MapSpan>& spans, cudaStream_t st) {
   // the books first: all of it, or none
   std::vector<PageMapping> maps(spans.size());
   auto undo = [&](size_t n) {
-    while (n-- > 0)
-      if (!spans[n].s->pool->priv) pages_unmap(*spans[n].s->pool, *spans[n].s, maps[n]);
+    while (n-- > 0) pages_unmap(*spans[n].s->pool, *spans[n].s, maps[n]);
   };
   for (size_t i = 0; i < spans.size(); ++i) {
     l3g_state* s = spans[i].s;
-    if (s->pool->priv ||
-        pages_map(*s->pool, *s, KV_PAGE, spans[i].pos0, spans[i].n_pos, s->high, maps[i]))
-      continue;
+    if (pages_map(*s->pool, *s, KV_PAGE, spans[i].pos0, spans[i].n_pos, s->high, maps[i])) continue;
     size_t want = maps[i].want;
     for (size_t j = 0; j < i; ++j)
       if (spans[j].s->pool == s->pool) want += maps[j].want;
@@ -595,6 +598,7 @@ int states_map(const std::vector<MapSpan>& spans, cudaStream_t st) {
 }
 
 int state_map(l3g_state* s, int pos0, int n_pos, cudaStream_t st) {
+  if (pages_ready(*s, KV_PAGE, pos0, n_pos)) return L3G_OK;
   return states_map({{s, pos0, n_pos}}, st);
 }
 
@@ -760,6 +764,8 @@ extern "C" int l3g_state_fork(const l3g_state* src, int32_t n_pos, int32_t ctx,
           s->h_pages[(size_t)h * s->pps + j] = id;
           ++p->refs[id];
         }
+      src->own_from = std::max(src->own_from, pages);
+      s->own_from = pages;
     }
     std::vector<int> table(s->h_pages);
     for (int& id : table) id = std::max(id, 0);
@@ -790,6 +796,7 @@ extern "C" int l3g_state_trim(l3g_state* s) {
       p->drop(id);
       id = -1;
     }
+  s->own_from = std::min(s->own_from, keep);
   s->mapped = keep;  // (the device table's entries behind it are not read)
   return L3G_OK;
 }

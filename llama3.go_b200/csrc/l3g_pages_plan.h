@@ -29,18 +29,29 @@ struct PageTable {
   int pps = 0;               // pages per (layer, kv head)
   std::vector<int> h_pages;  // -1: not mapped
   int mapped = 0;            // pages [0, mapped) of every (layer, kv head) are mapped
+  // pages [own_from, mapped) are mapped by this state alone, as far as is known
+  // without a look at their counts (a fork of the state raises it)
+  mutable int own_from = 0;
   int heads() const { return pps ? (int)(h_pages.size() / pps) : 0; }
 };
 
 // One state's part of making positions writable, and what undoes it.
 struct PageMapping {
   size_t want = 0;                // pages that it takes
-  int mapped0 = 0;                // the table's `mapped` before
+  int mapped0 = 0, own0 = 0;      // the table's `mapped` and `own_from` before
   int first = 0, last = 0;        // the table's columns that changed
   std::vector<size_t> entries;    // entries whose page others map too, and their
   std::vector<int> src, dst;      // page, the state's own copy of it
   std::vector<int> rows;          // and the rows of it that have been written
 };
+
+// Whether positions [pos0, n_pos) are writable as they are: what a step of a
+// state finds, but for one in KV_PAGE, without the pool's lock or a walk over
+// its pages' counts (64 sessions of 32 layers and 8 kv heads: 16384 of them).
+inline bool pages_ready(const PageTable& t, int page, int pos0, int n_pos) {
+  const int need = std::min(t.pps, (n_pos + page - 1) / page);
+  return need <= t.mapped && (pos0 / page >= t.own_from || pos0 / page >= need);
+}
 
 // Makes positions [pos0, n_pos) of table t writable: maps pages for positions
 // [0, n_pos), and replaces those of [pos0, n_pos) that other states map too by
@@ -52,6 +63,7 @@ inline bool pages_map(PageBook& book, PageTable& t, int page, int pos0, int n_po
   const int heads = t.heads(), need = std::min(t.pps, (n_pos + page - 1) / page);
   m = PageMapping{};
   m.mapped0 = m.first = t.mapped;
+  m.own0 = t.own_from;
   m.last = std::max(t.mapped, need);
   for (int j = pos0 / page; j < std::min(need, t.mapped); ++j)
     for (int h = 0; h < heads; ++h)
@@ -70,6 +82,7 @@ inline bool pages_map(PageBook& book, PageTable& t, int page, int pos0, int n_po
   }
   for (int j = t.mapped; j < need; ++j)
     for (int h = 0; h < heads; ++h) t.h_pages[(size_t)h * t.pps + j] = book.take();
+  if (std::min(need, t.mapped) >= t.own_from) t.own_from = std::min(t.own_from, pos0 / page);
   t.mapped = m.last;
   return true;
 }
@@ -85,6 +98,7 @@ inline void pages_unmap(PageBook& book, PageTable& t, const PageMapping& m) {
       id = -1;
     }
   t.mapped = m.mapped0;
+  t.own_from = m.own0;
   for (size_t i = m.entries.size(); i-- > 0;) {
     t.h_pages[m.entries[i]] = m.src[i];
     ++book.refs[m.src[i]];

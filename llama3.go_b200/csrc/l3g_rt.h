@@ -188,7 +188,7 @@ struct MapSpan {
   l3g_state* s;
   int pos0, n_pos;
 };
-int states_map(const std::vector<MapSpan>& spans, cudaStream_t st);  // l3g_model.cu
+int states_map(std::vector<MapSpan> spans, cudaStream_t st);  // l3g_model.cu
 int state_map(l3g_state* s, int pos0, int n_pos, cudaStream_t st);   // of one state
 // The error words of the serving operators' handles (l3g_ops.cu).
 Result* chunk_attn_word(l3g_chunk_attn* h);

@@ -15,6 +15,7 @@ constexpr int PAGE = 4, HEADS = 2, PPS = 5;
 
 struct State : PageTable {
   int pos = 0, high = 0;
+  bool alone = true;       // neither a fork nor forked
   std::vector<int> holds;  // what it wrote at each position
 };
 
@@ -32,7 +33,7 @@ bool same(const PageBook& a, const PageBook& b) {
   return a.free_pages == b.free_pages && a.refs == b.refs;
 }
 bool same(const PageTable& a, const PageTable& b) {
-  return a.h_pages == b.h_pages && a.mapped == b.mapped && a.pps == b.pps;
+  return a.h_pages == b.h_pages && a.mapped == b.mapped && a.pps == b.pps && a.own_from == b.own_from;
 }
 
 int fail(const char* what) {
@@ -50,6 +51,8 @@ int check(const World& w) {
         const int id = t.h_pages[h * PPS + j];
         if ((id >= 0) != (j < t.mapped)) return fail("a table entry without its page");
         if (id >= 0) ++refs[id];
+        if (id >= 0 && j >= t.own_from && w.book.refs[id] != 1)
+          return fail("a page taken for the state's own that others map");
       }
     for (int p = 0; p < t.pos; ++p)
       for (int h = 0; h < HEADS; ++h)
@@ -71,7 +74,17 @@ int batch(World& w, const std::vector<std::pair<int, int>>& who, int& stamp, boo
   size_t done = 0;
   for (; done < who.size(); ++done) {
     State& s = w.states[who[done].first];
-    if (!pages_map(w.book, s, PAGE, s.pos, s.pos + who[done].second, s.high, maps[done])) break;
+    const bool ready = pages_ready(s, PAGE, s.pos, s.pos + who[done].second);
+    if (s.alone && ready != (s.pos + who[done].second <= s.mapped * PAGE))
+      return fail("a state that was never forked: ready once its positions are mapped");
+    if (!pages_map(w.book, s, PAGE, s.pos, s.pos + who[done].second, s.high, maps[done])) {
+      if (ready) return fail("ready, and no pages");
+      break;
+    }
+    if (ready && maps[done].want) return fail("ready, and not writable");
+    if (!pages_ready(s, PAGE, s.pos, s.pos + who[done].second) &&
+        (s.pos + who[done].second + PAGE - 1) / PAGE >= s.own_from)
+      return fail("not ready behind its mapping");
   }
   if (done < who.size() || give_up) {
     while (done-- > 0) pages_unmap(w.book, w.states[who[done].first], maps[done]);
@@ -127,6 +140,9 @@ int run(unsigned seed) {
           if (j < f.mapped) ++w.book.refs[id];
           else id = -1;
         }
+      s.own_from = std::max(s.own_from, f.mapped);
+      f.own_from = f.mapped;
+      s.alone = f.alone = false;
       w.states[next++] = f;
     } else if (what == 2) {  // close
       for (int id : s.h_pages)
@@ -140,6 +156,7 @@ int run(unsigned seed) {
           w.book.drop(s.h_pages[h * PPS + j]);
           s.h_pages[h * PPS + j] = -1;
         }
+      s.own_from = std::min(s.own_from, keep);
       s.mapped = keep;
     } else if (what == 4) {  // back
       s.pos = rng() % (s.pos + 1);
