@@ -179,8 +179,9 @@ int l3g_state_pages(const l3g_state *s, int32_t *mapped);
  * trimmed) and continues from there; ctx_len <= 0 means src's.  In a shared
  * pool the two share the pages: nothing is copied until one of them writes to
  * a page that the other maps too, which then gives the writer a copy of its
- * own (a step that finds no free page for it fails with L3G_E_CTX).  A state
- * with a private pool is copied. */
+ * own (a step that finds no free page for it fails with L3G_E_CTX); once the
+ * pool has been freed its states cannot be forked.  A state with a private pool
+ * is copied. */
 int l3g_state_fork(const l3g_state *src, int32_t n_pos, int32_t ctx_len,
                    l3g_state **out);
 /* Gives the pages behind the state's position back to its shared pool (after
@@ -188,8 +189,9 @@ int l3g_state_fork(const l3g_state *src, int32_t n_pos, int32_t ctx_len,
 int l3g_state_trim(l3g_state *s);
 /* Moves the pages in use to the lowest ids, in the order of the states: then
  * the pages of a state's (layer, kv head) follow one another, and a snapshot
- * or a restore needs one copy for each.  No step of the pool's states may run.
- * *moved receives the pages that moved. */
+ * or a restore needs one copy for each.  No step, snapshot, restore or read of
+ * the pool's states may run meanwhile; states may be made, forked, trimmed and
+ * freed.  *moved receives the pages that moved. */
 int l3g_kvpool_compact(l3g_kvpool *p, int32_t *moved);
 int l3g_state_pos(const l3g_state *s, int32_t *pos);
 int l3g_state_ctx_len(const l3g_state *s, int32_t *ctx_len);

@@ -635,10 +635,10 @@ extern "C" int l3g_kvpool_free_pages(l3g_kvpool* p, int32_t* n) {
 extern "C" void l3g_state_free(l3g_state* s) {
   if (!s) return;
   cudaSetDevice(s->device);
+  if (s->pool) pool_leave(s->pool, s);  // (first: a compaction writes the members' tables)
   if (s->d_pages) cudaFree(s->d_pages);
   if (s->rope_cos) cudaFree(s->rope_cos);
   if (s->rope_sin) cudaFree(s->rope_sin);
-  if (s->pool) pool_leave(s->pool, s);
   delete s;
 }
 
@@ -671,8 +671,7 @@ static int state_create(l3g_model* m, l3g_kvpool* pool, int32_t ctx, l3g_state**
         l3g_state_free(s);
         return l3g_fail(L3G_E_INVALID, "KV pool already freed");
       }
-      ++pool->states;
-      pool->members.push_back(s);
+      ++pool->states;  // (a member once it is complete)
     }
     s->pool = pool;
     // unmapped entries point at page 0 until mapped: never read, since a
@@ -710,6 +709,10 @@ static int state_create(l3g_model* m, l3g_kvpool* pool, int32_t ctx, l3g_state**
   if (e != cudaSuccess) {
     l3g_state_free(s);
     return l3g_fail(L3G_E_CUDA, "state allocation: %s", cudaGetErrorString(e));
+  }
+  if (pool) {
+    std::lock_guard<std::mutex> lk(pool->mu);
+    pool->members.push_back(s);
   }
   *out = s;
   return L3G_OK;
@@ -756,21 +759,19 @@ extern "C" int l3g_state_fork(const l3g_state* src, int32_t n_pos, int32_t ctx,
     rc = copy_pages(s->pool, p->base, p->n_pages, s->pool->base, s->pool->n_pages, p->page_bytes,
                     from, to, rows, nullptr);
   } else {  // the pages are shared until one of the states writes to them
-    {
-      std::lock_guard<std::mutex> lk(p->mu);
-      for (int h = 0; h < heads; ++h)
-        for (int j = 0; j < pages; ++j) {
-          const int id = src->h_pages[(size_t)h * src->pps + j];
-          s->h_pages[(size_t)h * s->pps + j] = id;
-          ++p->refs[id];
-        }
-      src->own_from = std::max(src->own_from, pages);
-      s->own_from = pages;
-    }
-    std::vector<int> table(s->h_pages);
-    for (int& id : table) id = std::max(id, 0);
+    // (under the lock to the end: a compaction finds the state with none of its
+    // pages, or with all and a table that holds them)
+    std::lock_guard<std::mutex> lk(p->mu);
+    std::vector<int> table(s->h_pages.size(), 0);
+    for (int h = 0; h < heads; ++h)
+      for (int j = 0; j < pages; ++j) {
+        const int id = src->h_pages[(size_t)h * src->pps + j];
+        s->h_pages[(size_t)h * s->pps + j] = table[(size_t)h * s->pps + j] = id;
+        ++p->refs[id];
+      }
+    src->own_from = std::max(src->own_from, pages);
+    s->own_from = s->mapped = pages;
     e = cudaMemcpy(s->d_pages, table.data(), table.size() * sizeof(int), cudaMemcpyHostToDevice);
-    s->mapped = pages;
   }
   if (e != cudaSuccess) rc = l3g_fail(L3G_E_CUDA, "state fork: %s", cudaGetErrorString(e));
   if (rc) {

@@ -501,7 +501,8 @@ class KvPool:
 
     def Compact(self) -> int:
         """Moves the pages in use to the lowest ids, each state's in order;
-        returns how many moved.  No step of the pool's states may run."""
+        returns how many moved.  No step, snapshot, restore or read of the pool's
+        states may run meanwhile."""
         v = C.c_int32()
         _check(lib().l3g_kvpool_compact(self._h, C.byref(v)))
         return v.value

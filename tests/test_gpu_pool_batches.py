@@ -113,3 +113,65 @@ def test_a_fork_holds_only_what_its_source_ingested(gpu_lib):
     a.Fork(b.Pos).Close()
     for x in (a, b, ws, pool, m):
         x.Close()
+
+
+def test_states_come_and_go_while_a_pool_is_compacted(gpu_lib):
+    """Two threads make, fork, trim and free states of a pool that a third
+    compacts: nothing is lost, and the caches hold what they held."""
+    import threading
+
+    import synthetic
+    cfg, m, h = _load(gpu_lib)
+    ids = synthetic.prompt_ids(cfg, 500, seed=4)
+    batch = gpu_lib.Batch(m, 4)
+    pool = m.NewKvPool(12 * h)
+    roots = [m.NewStateInPool(pool, 512) for _ in range(3)]
+    for k in range(0, 300, 100):  # pages taken in turn
+        batch.extend(roots, [ids[k:k + 100]] * 3)
+    gone = m.NewStateInPool(pool, 512)
+    batch.extend([gone], [ids[:300]])
+    roots[0].Close()
+    roots = roots[1:]
+    snaps = [s.Snapshot() for s in roots]
+    free = pool.FreePages
+    errors = []
+
+    def churn(src, n):
+        try:
+            for i in range(n):
+                f = src.Fork(100 + 7 * i)
+                g = m.NewStateInPool(pool, 512)
+                f2 = f.Fork()
+                f.Pos = 50
+                f.Trim()
+                for s in (f, g, f2):
+                    s.Close()
+        except Exception as e:  # noqa: BLE001 - reported by the test's thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=churn, args=(s, 25)) for s in roots]
+    for t in threads:
+        t.start()
+    rounds = 0
+    while any(t.is_alive() for t in threads):
+        pool.Compact()
+        if rounds == 3:
+            gone.Close()
+        rounds += 1
+    for t in threads:
+        t.join()
+    assert not errors and rounds > 3
+    pool.Compact()
+    assert pool.FreePages == free + 2 * h
+    for s, snap in zip(roots, snaps):
+        assert np.array_equal(s.Snapshot(), snap)
+        own = m.NewState(512)
+        own.Restore(snap)
+        batch.extend([s], [ids[300:305]])
+        batch.extend([own], [ids[300:305]])
+        for layer in range(cfg.n_layers):
+            for got, want in zip(s.read_kv(layer, 0, 305), own.read_kv(layer, 0, 305)):
+                assert np.array_equal(got, want)
+        own.Close()
+    for s in roots + [batch, pool, m]:
+        s.Close()
