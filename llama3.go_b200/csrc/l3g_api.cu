@@ -14,6 +14,9 @@ int l3g_fail(int code, const char* fmt, ...) {
   vsnprintf(buf, sizeof buf, fmt, ap);
   va_end(ap);
   g_err = buf;
+  // the runtime keeps a failed call's error for the next look at it, which would
+  // be another call's check behind a launch
+  if (code == L3G_E_CUDA) cudaGetLastError();
   return code;
 }
 
