@@ -72,3 +72,47 @@ def test_magnitudes_differ_in_a_tile(gpu_lib, which):
     err = np.abs(got - want).max(axis=(0, 1))
     assert (err <= bound).all(), (err / bound).max()
     assert run.op.status() == (0, 0)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_pages_beyond_32_bits(gpu_lib, f16):
+    """Pages whose bytes lie beyond 2^32 in their pool, and rows of q and out
+    whose floats lie beyond 2^31: as pages and rows at the beginning.  The
+    same of l3g_kv_copy_pages, which brings them there."""
+    import torch
+    rng = np.random.default_rng(3)
+    n, kv, hd = 5, 700, 128
+    cache = Paged(rng, [(kv, 0)], 1, hd, f16, spare=0)
+    q = rng.normal(0, 1.3, (n, 4, hd)).astype(np.float32)
+    run = Run(gpu_lib, cache, [n], 4, q)
+    run()
+    want = run.got()[0]
+    small = run.pools[0]
+    page_bytes = small[0].numel() * small.element_size()
+    pages = (1 << 32) // page_bytes + 1000
+    big = torch.empty(pages, *small.shape[1:], dtype=small.dtype, device="cuda")
+    ids = lambda v: torch.tensor([int(i) for i in v], dtype=torch.int32, device="cuda")  # noqa: E731
+    have = cache.table[0, 0]
+    there = pages - 1 - np.arange(len(have))
+    status = torch.zeros(2, dtype=torch.int32, device="cuda")
+    src, dst = ids(have), ids(there)
+    gpu_lib.kv_copy_pages(small.data_ptr(), small.shape[0], big.data_ptr(), pages, page_bytes // ops_ref.PAGE,
+                          src.data_ptr(), dst.data_ptr(), 0, len(have), status.data_ptr())
+    torch.cuda.synchronize()
+    assert not status.any()
+    run.table.copy_(torch.from_numpy(there.astype(np.int32).reshape(cache.table.shape)))
+    run.desc[0]["pool"], run.desc[0]["n_pages"] = big.data_ptr(), pages
+    run.upload()
+    run.out.fill_(float("nan"))
+    run()
+    assert np.array_equal(run.got()[0], want) and run.op.status() == (0, 0)
+    # rows 2^29 floats apart
+    ld = 1 << 29
+    far = torch.empty(4 * ld + 1024, device="cuda")
+    for i in range(n):
+        far[i * ld:i * ld + 512] = torch.from_numpy(q[i].reshape(-1)).cuda()
+    run.op.run(run.seqs.data_ptr(), 1, n, far.data_ptr(), ld, far.data_ptr() + 2048, ld)
+    torch.cuda.synchronize()
+    for i in range(n):
+        assert np.array_equal(far[i * ld + 512:i * ld + 1024].cpu().numpy().reshape(4, hd), want[i])
+    assert run.op.status() == (0, 0)

@@ -68,3 +68,44 @@ def test_infinite_and_nan_slices(gpu_lib):
     for r in range(4):
         assert np.isnan(o["lp"][r]) and np.isnan(o["ent"][r]) and np.isnan(o["tlp"][r]).all(), r
     assert o["rank"][1] == 4 and np.array_equal(o["ids"][1], 2 * SLICE + np.arange(3))
+
+
+@pytest.mark.parametrize("v,k", [(170001, 64), (300000, 40), (600001, 64)])
+def test_many_slices(gpu_lib, v, k):
+    """More keys of the slices than are compared with each other (1024), and
+    than shared memory holds (2048): places by search in the slices' lists."""
+    rng = np.random.default_rng(v)
+    x = rng.normal(0, 3, (5, v)).astype(np.float32)
+    x[1] = rng.integers(0, 4, v)             # ties over every slice
+    x[2] = np.arange(v)                      # all alternatives in the last slice
+    x[3] = -np.arange(v)                     # in the first
+    x[4] = -np.inf
+    x[4, ::9000] = 1.0                       # fewer than k beside the masked
+    t = [7, v - 1, v - 2, 3, 9000]
+    o = _run(gpu_lib, x, t, k)
+    for r in range(5):
+        lp, ent, rank, ids, tlp = ops_ref.logprobs(x[r], t[r], k)
+        # (a row of 600000 distinct whole numbers: what counts spreads over 20)
+        assert abs(o["lp"][r] - lp) <= 2.0 ** -19 + 2.0 ** -22 * max(20.0, abs(lp)), (r, o["lp"][r], lp)
+        assert abs(o["ent"][r] - ent) <= 2.0 ** -19 + 2.0 ** -22 * 80, (r, o["ent"][r], ent)
+        assert o["rank"][r] == rank and np.array_equal(o["ids"][r], ids), r
+        np.testing.assert_allclose(o["tlp"][r], tlp, rtol=2.0 ** -21, atol=2.0 ** -17)
+
+
+def test_rows_beyond_32_bits(gpu_lib):
+    """Logits of more than 2^31 bytes times 2: the last rows as the first."""
+    import torch
+    v, n = 128256, 8400  # 4.3 GB
+    x = torch.randn(n, v, device="cuda") * 2
+    t = torch.arange(n, dtype=torch.int32, device="cuda") * 3
+    lp, ent = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    ids = torch.empty(n, 3, dtype=torch.int32, device="cuda")
+    op = gpu_lib.LogProbs(n, v)
+    op.run(x.data_ptr(), v, n, t.data_ptr(), lp.data_ptr(), ent.data_ptr(), 0, 3, ids.data_ptr())
+    assert op.status() == (0, 0)
+    for r in (0, 4186, 8373, 8374, 8399):
+        row = x[r].cpu().numpy()
+        a, b, _, c, _ = ops_ref.logprobs(row, 3 * r, 3)
+        assert abs(lp[r].item() - a) <= 2.0 ** -19 + 2.0 ** -22 * 40
+        assert abs(ent[r].item() - b) <= 2.0 ** -19 + 2.0 ** -22 * 80
+        assert np.array_equal(ids[r].cpu().numpy(), c)
