@@ -68,6 +68,8 @@ constexpr int CHUNK_MIN_KEYS = 128;
 // 350 / 322 / 316, 7 x 300 tokens 44.8 / 45.0 / 43.3.)
 constexpr int CHUNK_OPEN = 6;
 __host__ __device__ constexpr int chunk_min_tiles(int bn) { return CHUNK_MIN_KEYS / bn; }
+// the weights' scale, 2^13, and its inverse
+constexpr float CHUNK_P_EXP = 13.0f, CHUNK_P_UP = 8192.0f, CHUNK_P_DOWN = 1.0f / 8192.0f;
 // tensor-memory columns: scores / weights of the two groups (at most 128
 // each), q hi and lo (64 each), the tile output
 constexpr uint32_t CHUNK_T_S = 0, CHUNK_T_Q = 256, CHUNK_T_O = 384, CHUNK_T_COLS = 512;
@@ -352,7 +354,7 @@ __device__ __forceinline__ void chunk_row_slow(const KT* rows, int n, const floa
     float s = 0.0f;
 #pragma unroll 1
     for (int d = 0; d < HD; ++d) s = fmaf(q[d], (float)k[d], s);
-    const float p = ex2(fmaf(s, scale, 13.0f - (m == -INFINITY ? 0.0f : m)));
+    const float p = ex2(fmaf(s, scale, m == -INFINITY ? 0.0f : -m));
 #pragma unroll 1
     for (int d = 0; d < 16; ++d)
       o[d] = fmaf(p, (float)k[HD + chunk_dim(HD, (int)sizeof(KT), d0 + d)], o[d]);
@@ -426,7 +428,7 @@ __device__ __forceinline__ void chunk_rows_again(const ChunkArgs& a, const Chunk
       if (!good) break;
       const float mn = fmaxf(M, warp_max(s)), mu = mn == -INFINITY ? 0.0f : mn;
       const float f = M == -INFINITY ? 0.0f : ex2(M - mu);
-      const float p = ex2(s - mu + 13.0f);  // (the scale of the segment's weights)
+      const float p = ex2(s - mu);
       L = fmaf(L, f, warp_sum(p));
       M = mn;
 #pragma unroll
@@ -879,7 +881,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                 if (odd) {
                   chunk_row_slow<HD, KT>(rows, in ? seen : 0, qrow, a.scale, mt, dc, tb + lane * 20);
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(tb[lane * 20 + i] / vs);
+                  for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(tb[lane * 20 + i] / vs * CHUNK_P_UP);
                 }
                 __syncwarp();
                 tmem_st16(t_o + dc, v);
@@ -889,7 +891,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           }
           const float mn = fmaxf(M, mt);
           const float co = M == -INFINITY ? 0.0f : ex2(M - mn);
-          const float ct = mt == -INFINITY ? 0.0f : ex2(mt - mn) * vs;
+          // (the weights' scale goes here, or finite outputs of an f32 cache's
+          // largest values would pass fp32's range)
+          const float ct = mt == -INFINITY ? 0.0f : ex2(mt - mn) * (vs * CHUNK_P_DOWN);
           M = mn;
           const unsigned long long co2 = pk2(co, co), ct2 = pk2(ct, ct);
           const bool same = __all_sync(0xffffffffu, co == 1.0f);
@@ -922,7 +926,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const float mg = sh->m_team[g & 1][row];
-        L = fmaf(sh->l_group[g][row], mg == -INFINITY ? 0.0f : ex2(mg - M), L);
+        L = fmaf(sh->l_group[g][row], mg == -INFINITY ? 0.0f : ex2(mg - M) * CHUNK_P_DOWN, L);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->e_done);
@@ -1146,7 +1150,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           l *= m == -INFINITY ? 0.0f : ex2(m - mu);
           m = mn;
           if (half == 0) sh->m_tile[tile & 3][row] = m;
-          const float off = 13.0f - mu;
+          const float off = CHUNK_P_EXP - mu;
           const unsigned long long ks2 = pk2(ks, ks), off2 = pk2(off, off);
           const unsigned long long neg2 = pk2(-1.0f, -1.0f);
           unsigned long long sum = 0ull;  // a pair of fp32

@@ -116,3 +116,30 @@ def test_pages_beyond_32_bits(gpu_lib, f16):
     for i in range(n):
         assert np.array_equal(far[i * ld + 512:i * ld + 1024].cpu().numpy().reshape(4, hd), want[i])
     assert run.op.status() == (0, 0)
+
+
+@pytest.mark.parametrize("mag", [1e36, 1e-36])
+@pytest.mark.parametrize("unseen", [False, True])
+def test_values_near_the_ends_of_the_range(gpu_lib, mag, unseen):
+    """V so large that the weights' own scale (2^13) would take a finite mean
+    beyond fp32, and as small; also where a row's tile is taken again for an
+    unseen NaN."""
+    rng = np.random.default_rng(10)
+    n, kv = 9, 100
+    cache = Paged(rng, [(kv, 0)], 1, 64, False)
+    q = rng.normal(0, 1.3, (n, 4, 64)).astype(np.float32)
+    cache.v[0] *= np.float32(mag)
+    for p in cache.pools:
+        p[:, :, 1] *= np.float32(mag)
+    run = Run(gpu_lib, cache, [n], 4, q)
+    if unseen:
+        run.pools[0][cache.table[0, 0, 0], kv - 1, 1, 3] = float("nan")
+    run()
+    got = run.got()[0]
+    want = ops_ref.attention(q, (cache.k[0], cache.v[0]), n, kv)
+    bound = ops_ref.attention_bound(q, (cache.k[0], cache.v[0]))
+    assert np.abs(got[:-1] - want[:-1]).max() <= bound
+    last = np.abs(got[-1] - want[-1])
+    assert np.isnan(last[:, 3]).all() if unseen else last.max() <= bound
+    assert np.delete(last, 3, 1).max() <= bound
+    assert run.op.status() == (0, 0)

@@ -81,3 +81,21 @@ def test_infinite_query(f16, bad):
     assert err == 0 and np.isnan(got[2, 1]).all()
     got[2, 1] = want[2, 1]
     assert np.abs(got - want).max() <= ops_ref.attention_bound(q, (cache.k[0], cache.v[0]))
+
+
+@pytest.mark.parametrize("mag", [1e36, 1e-36])
+def test_values_near_the_ends_of_the_range(mag):
+    """V so large that the weights' own scale (2^13) would take a finite mean
+    beyond fp32, and as small."""
+    rng = np.random.default_rng(10)
+    n, kv = 5, 70
+    cache = Paged(rng, [(kv, 0)], 1, 32, False)
+    q = rng.normal(0, 1.3, (n, 2, 32)).astype(np.float32)
+    cache.v[0] *= np.float32(mag)
+    for p in cache.pools:
+        p[:, :, 1] *= np.float32(mag)
+    want = ops_ref.attention(q, (cache.k[0], cache.v[0]), n, kv)
+    for grid in (1, 2):
+        out, err, _ = simt_ops_lib.chunk_attention(cache, [n], 2, q, grid=grid)
+        got = out[:n].reshape(n, 2, 32)
+        assert err == 0 and np.abs(got - want).max() <= ops_ref.attention_bound(q, (cache.k[0], cache.v[0]))
