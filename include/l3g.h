@@ -548,8 +548,8 @@ int l3g_chunk_attn_new(int32_t n_heads, int32_t n_heads_kv, int32_t head_dim,
 void l3g_chunk_attn_free(l3g_chunk_attn *h);
 /* seqs: n_seqs descriptors (DEVICE, at most L3G_CHUNK_SEQS_MAX); total_q rows
  * of q (f32 [n_heads][head_dim] at q + row * ldq) and out (ldo), row strides in
- * floats, multiples of 4; layer selects the page-table rows; scale <= 0 means
- * 1 / sqrt(head_dim).  A descriptor outside its bounds (rows, kv_len, a page
+ * floats, multiples of 4, q and out apart in memory; layer selects the page-table
+ * rows; scale <= 0 means 1 / sqrt(head_dim).  A descriptor outside its bounds (rows, kv_len, a page
  * id) is skipped, its rows left as they were (for a bad page: those of the
  * head's tokens that see it, at least), and noted for l3g_chunk_attn_status.
  * A NaN in q gives NaN in its row, one in K or V in the rows that see it, and

@@ -13,20 +13,21 @@
 // rate for the one that a plain f16 attention takes, and the tiles follow each
 // other at 2700 to 3400, the time that two alternating tiles need for scores,
 // weights and output; 8 chunks of 1000 tokens after 7000: 2.1 to 2.3 ms, 430 to
-// 470 TFLOP/s at the 1.35 to 1.5 GHz that the power limit leaves.  64 decode
+// 470 TFLOP/s at the 1.35 to 1.5 GHz that the power limit leaves (each row tile
+// reads its cache anew: 6.4 GB from memory, 42% of its rate).  64 decode
 // steps after 512 to 8192: 300 to 320 us, 4.0 to 4.2 TB/s; of a tile's 128 rows 4
 // are used, and one of the four schedulers does all of its exponentials.  f32
 // caches: the loaders' conversion, 5000 cycles per tile and warp; 24 ragged
-// sessions 194 us.  Short calls: the chain of latencies of a row tile, about
+// sessions 188 to 196 us.  Short calls: the chain of latencies of a row tile, about
 // 10000 cycles (8 us) to its first output; one token 22 us.
 //
 // Precision.  q, out and the statistics are fp32; the products run on the f16
 // tensor cores.  An fp32 operand x goes in as two f16 terms, hi = f16(x) and
 // lo = f16(x - hi), after scaling by a power of two (exact, undone in fp32), so
-// it keeps 22 bits: q scaled per row, the weights p by 2^13, the K and V tiles
-// of an f32 cache per tile; f16 caches go in as they are.  An f16 cache takes
-// two products per tile (hi K, lo K), an f32 cache three (the lo lo term is
-// below 2^-22).  The accumulators of one tile are fp32 in tensor memory; the
+// it keeps 22 bits: q scaled per row, the weights p by 2^13 (taken out again where
+// a tile's output joins the sums), the K and V tiles of an f32 cache per tile; f16
+// caches go in as they are.  An f16 cache takes two products per tile (hi K,
+// lo K), an f32 cache three (the lo lo term is below 2^-22).  The accumulators of one tile are fp32 in tensor memory; the
 // sum over tiles is fp32 in registers, rounded to nearest, because the tensor
 // core's own accumulation truncates and a long cache would add that up.
 #pragma once
