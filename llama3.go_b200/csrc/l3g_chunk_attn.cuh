@@ -117,7 +117,8 @@ struct ChunkSmem {
   uint64_t qx[4], mx[2][4];
   uint32_t tmem_base;
   int abort_flag;
-  int n_tiles_lo, pad;
+  int alive;                     // changes while rows are taken again: nothing hangs
+  int pad;
   long long begin, end;          // the CTA's range of the linear order
   long long unit0;               // where the row tile that holds `begin` begins
   int s0, kvh0, rt0, pad0;
@@ -177,16 +178,21 @@ __host__ __device__ constexpr int chunk_smem_bytes(int hd, int es) {
 // Bounded wait of a whole warp, for waits that are on the critical path many
 // times: no divergence, the warp suspended by the hardware (polling warps
 // would take issue slots from the others) for 20 us a try, and the timer, which
-// takes longer to read than most of the waits, looked at every 16th try.
+// takes longer to read than most of the waits, looked at every 16th try.  The
+// bound counts from the last sign of chunk_rows_again, which is longer at work
+// the longer the cache is.
 __device__ __forceinline__ bool chunk_wait(uint64_t* b, uint32_t parity, ChunkSmem* sh,
                                            const ChunkArgs& a, int where) {
   uint64_t t0 = 0;
+  int alive = 0;
   for (int i = 0;; ++i) {
     if (__all_sync(0xffffffffu, mbar_try_wait(b, parity, 20000))) return true;
     if (__any_sync(0xffffffffu, *(volatile int*)&sh->abort_flag)) return false;
     if ((i & 15) == 15) {
       const uint64_t t = gtime();
-      if (t0 == 0) t0 = t;
+      const int sign = *(volatile int*)&sh->alive;
+      if (t0 == 0 || sign != alive) t0 = t;
+      alive = sign;
       if (__any_sync(0xffffffffu, t - t0 > a.wait_ns)) {
         *(volatile int*)&sh->abort_flag = 1;
         if ((threadIdx.x & 31) == 0) report(a.res, ERR_TIMEOUT, where);
@@ -384,45 +390,102 @@ __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(
 // K comes as NaN from two-term operands (its lo term, or a q term that is zero
 // or has the other sign), where a score of -inf weighs nothing.  A row with a
 // score that is NaN or +inf, or with a q that is not finite, stays NaN, as it
-// was written.  It hardly ever runs (32 rows over 128 Ki keys: below the waits'
-// bound, which the other warps' waits for this one have to keep).
+// was written.  It hardly ever runs and is not made to be fast: one such key that
+// all rows of 600 tokens see after 131072 positions (32 query and 8 kv heads of
+// 128) costs 0.55 s, f32 1.3 s, where the call takes 2.4 and 5.1 ms.  The other
+// warps' waits last that long, so it shows them that it is at work (alive).
 template <int HD, typename KT>
 __device__ __forceinline__ void chunk_rows_again(const ChunkArgs& a, const ChunkCursor& c,
                                                  uint32_t rows, int quarter, int lane, bool split,
-                                                 size_t place) {
-  constexpr int V = HD / 32, BN = chunk_bn((int)sizeof(KT));
+                                                 size_t place, int* alive) {
+  constexpr int V = HD / 32, BN = chunk_bn((int)sizeof(KT)), W = 16 / (int)sizeof(KT);
+  struct alignas(16) Piece {
+    KT x[W];
+  };
+  struct alignas(V * sizeof(KT)) Dims {
+    KT x[V];
+  };
   const int tt = CHUNK_BM / a.group;
   const int* pages = c.q.pages + ((size_t)a.layer * a.hkv + c.kvh) * c.q.pps;
+  // the keys from kb on, up to the page's end; null for a page outside its pool
+  auto cells_at = [&](int kb) -> const KT* {
+    if ((kb & (KV_PAGE - 1)) == 0 && lane == 0) ++*(volatile int*)alive;
+    const int page = pages[kb / KV_PAGE];
+    if (page < 0 || page >= c.q.n_pages) return nullptr;
+    return reinterpret_cast<const KT*>(c.q.pool) +
+           ((size_t)page * KV_PAGE + (kb & (KV_PAGE - 1))) * 2 * HD;
+  };
+  auto q_at = [&](int row) {
+    const int tok = row * a.ginv >> 16;
+    return a.q + ((long long)c.q.q0 + (long long)c.rt * tt + tok) * a.ldq +
+           (size_t)(c.kvh * a.group + row - tok * a.group) * HD;
+  };
+  // rows with a finite q, and the first keys with a NaN and with an infinity:
+  // a row that sees the one stays NaN, one that does not see the other too
+  uint32_t left = 0;
 #pragma unroll 1
   for (; rows; rows &= rows - 1) {
-    const int row = quarter * 32 + __ffs(rows) - 1, tok = row * a.ginv >> 16;
+    const float* q = q_at(quarter * 32 + __ffs(rows) - 1) + lane * V;
+    bool good = true;
+#pragma unroll
+    for (int i = 0; i < V; ++i) good = good && fabsf(q[i]) <= 3.4028235e38f;
+    if (__all_sync(0xffffffffu, good)) left |= rows & (0u - rows);
+  }
+  const int last = min(c.j1 * BN, c.q.kv_len);
+  int nan_at = last, inf_at = last;
+#pragma unroll 1
+  for (int kb = c.j0 * BN; kb < last && left && nan_at == last; kb += 32) {  // (32 divides a page)
+    const KT* cells = cells_at(kb);
+    if (!cells) return;
+    bool nan = false, inf = false;
+    if (kb + lane < last) {
+#pragma unroll 4
+      for (int d = 0; d < HD; d += W) {
+        const Piece x = *reinterpret_cast<const Piece*>(cells + (size_t)lane * 2 * HD + d);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          const float f = (float)x.x[i];
+          nan = nan || f != f;
+          inf = inf || fabsf(f) > 3.4028235e38f;
+        }
+      }
+    }
+    const uint32_t bn = __ballot_sync(0xffffffffu, nan), bi = __ballot_sync(0xffffffffu, inf);
+    if (bn) nan_at = kb + __ffs(bn) - 1;
+    if (bi && inf_at == last) inf_at = kb + __ffs(bi) - 1;
+  }
+#pragma unroll 1
+  for (; left; left &= left - 1) {
+    const int row = quarter * 32 + __ffs(left) - 1, tok = row * a.ginv >> 16;
     const long long at = (long long)c.q.q0 + (long long)c.rt * tt + tok;
     const int head = c.kvh * a.group + row - tok * a.group;
-    const float* q = a.q + at * a.ldq + (size_t)head * HD;
+    const float* q = q_at(row);
     const int end = min(c.j1 * BN, c.q.kv_len - c.q.n_q + c.rt * tt + tok + 1);
+    if (end > nan_at || end <= inf_at) continue;
     float M = -INFINITY, L = 0.0f, o[V];
     bool good = true;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      o[i] = 0.0f;
-      good = good && fabsf(q[lane * V + i]) <= 3.4028235e38f;
-    }
-    good = __all_sync(0xffffffffu, good);
+    for (int i = 0; i < V; ++i) o[i] = 0.0f;
 #pragma unroll 1
-    for (int kb = c.j0 * BN; kb < end && good; kb += 32) {  // (32 divides a page)
-      const int page = pages[kb / KV_PAGE], cnt = min(32, end - kb);
-      good = page >= 0 && page < c.q.n_pages;
-      if (!good) break;
-      const KT* cells = reinterpret_cast<const KT*>(c.q.pool) +
-                        ((size_t)page * KV_PAGE + (kb & (KV_PAGE - 1))) * 2 * HD;
+    for (int kb = c.j0 * BN; kb < end && good; kb += 32) {
+      const int cnt = min(32, end - kb);
+      const KT* cells = cells_at(kb);
       float s = -INFINITY;
       if (lane < cnt) {
         const KT* k = cells + (size_t)lane * 2 * HD;
         float d4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-        for (int d = 0; d < HD; d += 4)
+        for (int d = 0; d < HD; d += W) {
+          const Piece x = *reinterpret_cast<const Piece*>(k + d);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) d4[i] = fmaf(q[d + i], (float)k[d + i], d4[i]);
+          for (int i = 0; i < W; i += 4) {
+            const float4 y = *reinterpret_cast<const float4*>(q + d + i);
+            d4[0] = fmaf(y.x, (float)x.x[i], d4[0]);
+            d4[1] = fmaf(y.y, (float)x.x[i + 1], d4[1]);
+            d4[2] = fmaf(y.z, (float)x.x[i + 2], d4[2]);
+            d4[3] = fmaf(y.w, (float)x.x[i + 3], d4[3]);
+          }
+        }
         s = ((d4[0] + d4[1]) + (d4[2] + d4[3])) * a.scale;
       }
       good = __all_sync(0xffffffffu, s < INFINITY);
@@ -437,9 +500,9 @@ __device__ __forceinline__ void chunk_rows_again(const ChunkArgs& a, const Chunk
 #pragma unroll 8
       for (int j = 0; j < cnt; ++j) {
         const float pj = __shfl_sync(0xffffffffu, p, j);
-        const KT* v = cells + (size_t)j * 2 * HD + HD + lane * V;
+        const Dims v = *reinterpret_cast<const Dims*>(cells + (size_t)j * 2 * HD + HD + lane * V);
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = fmaf(pj, (float)v[i], o[i]);
+        for (int i = 0; i < V; ++i) o[i] = fmaf(pj, (float)v.x[i], o[i]);
       }
     }
     if (!good) continue;
@@ -516,7 +579,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     mbar_init(&sh->l_full, CHUNK_SOFT);
     mbar_init(&sh->e_done, CHUNK_OUT);
     mbar_init(&sh->drain, 1);
-    sh->abort_flag = 0;
+    sh->abort_flag = sh->alive = 0;
     for (int i = 0; i < 16; ++i) sh->bad[i] = 0;
     fence_mbar_init();
     mbar_arrive(&sh->s_go[0]);  // nothing lies over the first two S
@@ -976,7 +1039,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         const uint32_t again = __ballot_sync(0xffffffffu, live && !bad && L != L);
         if (again) {
           __syncwarp();  // (over what other lanes have written)
-          chunk_rows_again<HD, KT>(a, c, again, quarter, lane, split, place);
+          chunk_rows_again<HD, KT>(a, c, again, quarter, lane, split, place, &sh->alive);
         }
       }
       if (warp == CHUNK_WARP_OUT && lane == 0 && split && c.j1 == c.nk) {

@@ -74,3 +74,37 @@ def test_infinite_query(gpu_lib, f16, bad):
     want = ops_ref.attention(q, (cache.k[0], cache.v[0]), n, kv)
     got[17, 1] = want[17, 1]
     assert np.abs(got - want).max() <= ops_ref.attention_bound(q, (cache.k[0], cache.v[0]))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_infinite_key_of_a_long_cache(gpu_lib, f16):
+    """Every row of many row tiles taken again over 131072 positions, which takes
+    longer than other waits of the kernel may: no wait gives up."""
+    import torch
+    heads, hkv, hd, n, kv = 32, 8, 128, 600, 131072
+    g = torch.Generator(device="cuda").manual_seed(1)
+    pps = kv // PAGE
+    pool = torch.empty(hkv * pps, PAGE, 2, hd, dtype=torch.float16 if f16 else torch.float32, device="cuda")
+    for h in range(hkv):
+        pool[h * pps:(h + 1) * pps] = torch.randn(pps, PAGE, 2, hd, generator=g, device="cuda")
+    pool[::pps, 10, 0, 5] = -float("inf")
+    table = torch.arange(hkv * pps, dtype=torch.int32, device="cuda")
+    q = torch.randn(n, heads, hd, generator=g, device="cuda") * 1.3
+    q[..., 5] = q[..., 5].abs() + 0.01
+    out = torch.full_like(q, float("nan"))
+    desc = gpu_lib.chunk_seqs(1)
+    desc["pool"], desc["n_pages"], desc["pages"], desc["pps"] = pool.data_ptr(), hkv * pps, table.data_ptr(), pps
+    desc["n_q"], desc["kv_len"] = n, kv
+    sd = torch.from_numpy(desc.view(np.uint8)).cuda()
+    op = gpu_lib.ChunkAttention(heads, hkv, hd, gpu_lib.L3G_KV_F16 if f16 else gpu_lib.L3G_KV_F32)
+    op.run(sd.data_ptr(), 1, n, q.data_ptr(), heads * hd, out.data_ptr(), heads * hd)
+    assert op.status() == (0, 0)
+    assert torch.isfinite(out).all()
+    for t, h in ((0, 0), (123, 17), (599, 31)):
+        cells = pool[h // 4 * pps:(h // 4 + 1) * pps].reshape(kv, 2, hd)
+        see = kv - n + t + 1
+        K, V = cells[:see, 0].cpu().numpy()[None], cells[:see, 1].cpu().numpy()[None]
+        qi = q[t, h].cpu().numpy()[None, None]
+        want = ops_ref.attention(qi, (K, V), 1, see)
+        K[0, 10, 5] = 0  # (for the bound)
+        assert np.abs(out[t, h].cpu().numpy() - want[0, 0]).max() <= ops_ref.attention_bound(qi, (K, V))
